@@ -346,6 +346,92 @@ int natten_b200_merge_backward(int32_t dtype, int64_t rows, int32_t head_dim, co
                                const void* dout, const float* dlse, void* do0, float* dl0,
                                void* do1, float* dl1, void* stream);
 
+/*
+ * Layer norm over the last axis: y = (x - mean) / sqrt(var + eps) * weight + bias, statistics in float32.
+ * A tensor of `rows` rows of `channels` elements; row r of x starts (r / inner) * outer_stride +
+ * (r % inner) * inner_stride elements behind x, channels lie side by side.  So x may be, for instance, the queries
+ * inside the output of a fused q/k/v projection (rows = tokens * heads, inner = heads).  y, dy and dx are dense.
+ * weight and bias (nullable, [channels]) have the tensor's dtype or are float32 (weight_dtype).  mean and rstd (both or
+ * neither, float32 [rows]) keep what the backward needs.
+ *
+ * The backward writes dx (nullable) and dweight / dbias (nullable, in weight_dtype), the latter summed over the rows in
+ * an order that does not change from call to call.  scratch (4-byte aligned, at least
+ * natten_b200_layer_norm_backward_scratch_bytes) is needed when dweight or dbias is wanted.
+ * The blocks around the reference's modules norm their input so (src/natten_mlx/nn/na2d.py:14-154 is the layer in
+ * between); the reference leaves the norm to its array library.
+ */
+typedef struct natten_b200_rows {
+  int64_t rows;
+  int64_t inner;            /* 1: one stride, outer_stride, for all rows */
+  int64_t outer_stride, inner_stride;
+  int32_t channels;
+  int32_t reserved;         /* must be zero */
+} natten_b200_rows;
+int natten_b200_layer_norm_forward(int32_t dtype, int32_t weight_dtype, const natten_b200_rows* rows, const void* x,
+                                   const void* weight, const void* bias, float eps, void* y, float* mean, float* rstd,
+                                   void* stream);
+size_t natten_b200_layer_norm_backward_scratch_bytes(int64_t rows, int32_t channels);
+int natten_b200_layer_norm_backward(int32_t dtype, int32_t weight_dtype, const natten_b200_rows* rows, const void* x,
+                                    const void* weight, const float* mean, const float* rstd, const void* dy, void* dx,
+                                    void* dweight, void* dbias, void* scratch, size_t scratch_bytes, void* stream);
+
+/*
+ * Rotary positions: of the first sum(axis_dims) channels of every head of q and k, pair p turns by
+ * position[axis of p] * phases[p]; the other channels pass through.  Pairs are numbered axis by axis; pair p is
+ * channels (2p, 2p + 1) when interleaved, else (p, p + pairs).  phases[p] is the angle per position as a fraction of a
+ * turn times 2^64 (host array, read during the call).  inverse != 0 turns the other way: the gradient.
+ * q [batch, extent..., heads_q, head_dim] and k [.., heads_k, head_dim] may have any token and head stride (elements);
+ * yq and yk are dense.  The position of a token on axis a is
+ *   NATTEN_B200_POS_GRID     origin[a] plus its index on spatial axis a (n_axes == rank)
+ *   NATTEN_B200_POS_OFFSET   that plus positions[batch, a]: int32 or int64 [batch, rank] on the device
+ *   NATTEN_B200_POS_GIVEN    positions[token, a]: int32 or int64 [batch or 1, extent..., n_axes] on the device
+ *                            (position_batch == 0: one set of positions for all samples)
+ * Any position that fits 32 bits keeps its angle exactly (the angle wraps around at whole turns in integers).  No counterpart in
+ * the reference, whose positional term is the relative bias of its allin1 ops.
+ */
+enum { NATTEN_B200_POS_GRID = 0, NATTEN_B200_POS_OFFSET = 1, NATTEN_B200_POS_GIVEN = 2 };
+typedef struct natten_b200_rotary_geom {
+  int32_t dtype, rank;
+  int64_t batch;
+  int32_t extent[3];
+  int32_t heads_q, heads_k, head_dim;
+  int32_t n_axes, axis_dims[3];        /* 1..3 axes; even, their sum at most head_dim and 512 */
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride;
+  int32_t interleaved, position_kind, position_bits, position_batch;
+  int64_t origin[3];
+  const void* positions;
+  const uint64_t* phases;              /* host, [sum(axis_dims) / 2] */
+} natten_b200_rotary_geom;
+int natten_b200_rotary(const natten_b200_rotary_geom* g, const void* q, const void* k, void* yq, void* yk,
+                       int32_t inverse, void* stream);
+
+/*
+ * Attention of a batch's queries to one prefix that every sample shares:
+ * out = softmax(scale * q . k) . v over the prefix's tokens, lse the log-sum-exp of the same logits (nullable).
+ * q [batch, tokens, heads_q, head_dim], k and v [prefix, heads_kv, head_dim] with any token and head stride (elements);
+ * out [batch, tokens, heads_q, head_dim] and lse (float32) are dense.  The prefix is read once for the batch: the
+ * queries of a key/value head are the rows of one product.  lens (nullable, device, int32 [batch]) lets sample b see the
+ * first lens[b] tokens only; a row that sees none gets out 0 and lse -inf, and nothing that k or v hold past a sample's
+ * length reaches its rows.  With window_out / window_lse (both or neither: the same queries' result over other keys,
+ * such as natten_b200_fused_forward leaves) out and lse are those of the union of both sets of keys, as
+ * natten_b200_merge_forward would join them.  scratch: natten_b200_prefix_scratch_bytes, 16-byte aligned, may be null
+ * when that is 0.  Forward only.  bf16 / fp16 with head_dim a multiple of 8 up to 128 run on the tensor cores, the rest
+ * (head_dim up to 256) on the CUDA cores; path as in the fused entry points.  The extra tokens of the fused entry points
+ * belong to one sample each; the reference's composition for them is src/natten_mlx/functional.py:71-104.
+ */
+typedef struct natten_b200_prefix_geom {
+  int32_t dtype, heads_q, heads_kv, head_dim;
+  int64_t batch, tokens, prefix;
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  float scale;                         /* positive */
+  int32_t path;                        /* NATTEN_B200_PATH_* */
+  const int32_t* lens;
+} natten_b200_prefix_geom;
+size_t natten_b200_prefix_scratch_bytes(const natten_b200_prefix_geom* g);
+int natten_b200_prefix_forward(const natten_b200_prefix_geom* g, const void* q, const void* k, const void* v,
+                               const void* window_out, const float* window_lse, void* out, float* lse, void* scratch,
+                               size_t scratch_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -20,6 +20,8 @@ size_t fused_backward_scratch_sm100(const Geo& g, int dtype);
 int sm100_read_status();
 // Device address of the status word of the current device (nullptr without a device).
 int* sm100_status_word();
+// The driver's cuTensorMapEncodeTiled (nullptr when it is not available).
+void* sm100_encode_tiled();
 // Diagnostic builds (-DNB_SM100_PROFILE): buffer that receives the kernels' cycle counters.
 void sm100_set_profile_buffer(float* ptr);
 // Text description of the tiling chosen for a geometry (no GPU needed).

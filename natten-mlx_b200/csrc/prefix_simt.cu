@@ -1,0 +1,422 @@
+// Attention to a shared prefix on the CUDA cores (float32, and the head sizes that the tensor-core kernel does not
+// take), the kernel that joins the parts of a split prefix, and the entry point of both families.
+//
+//   out = softmax(scale q k^T) v,  lse = log sum exp(scale q k^T)
+//
+// One pass over the keys with a running maximum and sum per row.  A block holds BM rows of one key/value head and walks
+// its part of the prefix in tiles of BN keys: S = q k^T by 4x4 or smaller register tiles out of shared memory, the
+// probabilities through shared memory, O += P v in registers.  With many rows the float32 units bound it, with few the
+// reading of k and v, which then is spread over all SMs by splitting the prefix.
+#include <math.h>
+
+#include "prefix.cuh"
+
+namespace nb {
+namespace {
+
+constexpr int kSMs = 148;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// Four elements of a row from column c as float32; zeros past D and for rows that do not exist.
+template <typename T>
+__device__ __forceinline__ float4 load4(const T* row, int c, int D, bool vec, bool live) {
+  float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (!live) return r;
+  if (vec && c + 4 <= D) {
+    if constexpr (sizeof(T) == 4) {
+      r = *reinterpret_cast<const float4*>(row + c);
+    } else {
+      const uint2 raw = *reinterpret_cast<const uint2*>(row + c);
+      const T* e = reinterpret_cast<const T*>(&raw);
+      r = make_float4(to_f<T>(e[0]), to_f<T>(e[1]), to_f<T>(e[2]), to_f<T>(e[3]));
+    }
+  } else {
+    if (c < D) r.x = to_f<T>(row[c]);
+    if (c + 1 < D) r.y = to_f<T>(row[c + 1]);
+    if (c + 2 < D) r.z = to_f<T>(row[c + 2]);
+    if (c + 3 < D) r.w = to_f<T>(row[c + 3]);
+  }
+  return r;
+}
+
+// BM rows (RM = BM / 16 per thread), BN keys (CN = BN / 16 per thread), head dims up to 64 * NJ.
+template <typename T, int BM, int BN, int NJ>
+__global__ void __launch_bounds__(256) prefix_simt(const PrefixArgs a, bool vec) {
+  constexpr int RM = BM / 16, CN = BN / 16;
+  extern __shared__ float smem[];
+  const int Dp = (a.D + 3) & ~3, LD = Dp + 4;
+  float* qs = smem;                    // [BM][LD]
+  float* ks = qs + BM * LD;            // [BN][LD]
+  float* vs = ks + BN * LD;            // [BN][Dp]
+  float* ps = vs + BN * Dp;            // [BM][BN + 4]
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int hk = blockIdx.y;
+  const long long rows = a.tokens * a.G, row0 = (long long)blockIdx.x * BM;
+  const int tiles = (a.prefix + BN - 1) / BN;
+  const int t0 = (int)((long long)tiles * blockIdx.z / a.splits), t1 = (int)((long long)tiles * (blockIdx.z + 1) / a.splits);
+
+  for (int i = threadIdx.x; i < BM * (Dp / 4); i += 256) {
+    const int r = i / (Dp / 4), c = (i - r * (Dp / 4)) * 4;
+    const long long rr = row0 + r;
+    const bool live = rr < rows;
+    const long long tok = live ? rr / a.G : 0;
+    const int h = hk * a.G + (live ? (int)(rr - tok * a.G) : 0);
+    *reinterpret_cast<float4*>(qs + r * LD + c) =
+        load4<T>(static_cast<const T*>(a.q) + tok * a.q_token + (long long)h * a.q_head, c, a.D, vec, live);
+  }
+  float m[RM], l[RM];
+  float4 o[RM][NJ];
+  int lim[RM];
+  int most = 0;                        // no row of the block sees keys past it
+#pragma unroll
+  for (int i = 0; i < RM; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+    const long long rr = row0 + ty + 16 * i;
+    lim[i] = rr < rows ? prefix_limit(a, rr / a.G) : 0;
+    most = max(most, lim[i]);
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) o[i][j] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  const float sc = a.scale * kLog2e;
+  for (int t = t0; t < t1; ++t) {
+    const int key0 = t * BN;
+    if (!__syncthreads_or(most > key0)) break;       // also: the last tile's reads are over
+    for (int i = threadIdx.x; i < BN * (Dp / 4); i += 256) {
+      const int r = i / (Dp / 4), c = (i - r * (Dp / 4)) * 4;
+      const long long key = key0 + r;
+      const bool live = key < a.prefix;
+      *reinterpret_cast<float4*>(ks + r * LD + c) =
+          load4<T>(static_cast<const T*>(a.k) + (live ? key : 0) * a.k_token + (long long)hk * a.k_head, c, a.D, vec, live);
+      *reinterpret_cast<float4*>(vs + r * Dp + c) =
+          load4<T>(static_cast<const T*>(a.v) + (live ? key : 0) * a.v_token + (long long)hk * a.v_head, c, a.D, vec, live);
+    }
+    __syncthreads();
+    float s[RM][CN];
+#pragma unroll
+    for (int i = 0; i < RM; ++i)
+#pragma unroll
+      for (int j = 0; j < CN; ++j) s[i][j] = 0.f;
+    for (int d = 0; d < Dp; d += 4) {
+      float4 qv[RM], kv[CN];
+#pragma unroll
+      for (int i = 0; i < RM; ++i) qv[i] = *reinterpret_cast<const float4*>(qs + (ty + 16 * i) * LD + d);
+#pragma unroll
+      for (int j = 0; j < CN; ++j) kv[j] = *reinterpret_cast<const float4*>(ks + (tx + 16 * j) * LD + d);
+#pragma unroll
+      for (int i = 0; i < RM; ++i)
+#pragma unroll
+        for (int j = 0; j < CN; ++j)
+          s[i][j] = fmaf(qv[i].x, kv[j].x, fmaf(qv[i].y, kv[j].y, fmaf(qv[i].z, kv[j].z, fmaf(qv[i].w, kv[j].w, s[i][j]))));
+    }
+    bool whole = true;                   // every row of this thread sees every key of the tile
+#pragma unroll
+    for (int i = 0; i < RM; ++i) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < CN; ++j) {
+        s[i][j] = key0 + tx + 16 * j < lim[i] ? s[i][j] * sc : -INFINITY;
+        mx = fmaxf(mx, s[i][j]);
+      }
+#pragma unroll
+      for (int w = 8; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+      const float mn = fmaxf(m[i], mx), base = mn == -INFINITY ? 0.f : mn;
+      const float alpha = exp2f(m[i] - base);
+      m[i] = mn;
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < CN; ++j) {
+        const float p = exp2f(s[i][j] - base);
+        sum += p;
+        ps[(ty + 16 * i) * (BN + 4) + tx + 16 * j] = p;
+      }
+#pragma unroll
+      for (int w = 8; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+      l[i] = l[i] * alpha + sum;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) { o[i][j].x *= alpha; o[i][j].y *= alpha; o[i][j].z *= alpha; o[i][j].w *= alpha; }
+      whole = whole && lim[i] >= key0 + BN;
+    }
+    __syncwarp();                        // the 16 threads of a row are half a warp: ps of a row stays in its warp
+    if (whole || a.lens == nullptr) {
+#pragma unroll 1
+      for (int kk = 0; kk < BN; kk += 4) {
+        float4 pv[RM];
+#pragma unroll
+        for (int i = 0; i < RM; ++i) pv[i] = *reinterpret_cast<const float4*>(ps + (ty + 16 * i) * (BN + 4) + kk);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          const int c = tx * 4 + 64 * j;
+          if (c < Dp) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const float4 vv = *reinterpret_cast<const float4*>(vs + (kk + x) * Dp + c);
+#pragma unroll
+              for (int i = 0; i < RM; ++i) {
+                const float p = x == 0 ? pv[i].x : x == 1 ? pv[i].y : x == 2 ? pv[i].z : pv[i].w;
+                o[i][j].x = fmaf(p, vv.x, o[i][j].x);
+                o[i][j].y = fmaf(p, vv.y, o[i][j].y);
+                o[i][j].z = fmaf(p, vv.z, o[i][j].z);
+                o[i][j].w = fmaf(p, vv.w, o[i][j].w);
+              }
+            }
+          }
+        }
+      }
+    } else {
+      // a tile in which a row's keys end: values past the end stay out of the sum, whatever they hold
+#pragma unroll 1
+      for (int kk = 0; kk < BN; ++kk)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          const int c = tx * 4 + 64 * j;
+          if (c < Dp) {
+            const float4 vv = *reinterpret_cast<const float4*>(vs + kk * Dp + c);
+#pragma unroll
+            for (int i = 0; i < RM; ++i)
+              if (key0 + kk < lim[i]) {
+                const float p = ps[(ty + 16 * i) * (BN + 4) + kk];
+                o[i][j].x = fmaf(p, vv.x, o[i][j].x);
+                o[i][j].y = fmaf(p, vv.y, o[i][j].y);
+                o[i][j].z = fmaf(p, vv.z, o[i][j].z);
+                o[i][j].w = fmaf(p, vv.w, o[i][j].w);
+              }
+          }
+        }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < RM; ++i) {
+    const long long rr = row0 + ty + 16 * i;
+    if (rr >= rows) continue;
+    const long long tok = rr / a.G;
+    const long long at = tok * a.Hq + hk * a.G + (int)(rr - tok * a.G);
+    const float inv = l[i] > 0.f ? 1.f / l[i] : (l[i] == 0.f ? 0.f : l[i]);     // a NaN sum stays one
+    float lse = l[i] == 0.f ? -INFINITY : (m[i] + log2f(l[i])) * kLn2;
+    float wa = 1.f, wb = 0.f;
+    const bool last = a.splits == 1;
+    const bool win = last && a.window_lse != nullptr;
+    if (win) lse = join_weights(lse, a.window_lse[at], wa, wb);
+    const T* wo = static_cast<const T*>(a.window_out) + at * a.D;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const float f[4] = {o[i][j].x, o[i][j].y, o[i][j].z, o[i][j].w};
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int c = tx * 4 + 64 * j + x;
+        if (c < a.D) {
+          float v = f[x] * inv;
+          if (win) v = (wa != 0.f ? v * wa : 0.f) + (wb != 0.f ? to_f<T>(wo[c]) * wb : 0.f);
+          if (last) static_cast<T*>(a.out)[at * a.D + c] = from_f<T>(v);
+          else a.part_out[((long long)blockIdx.z * a.tokens * a.Hq + at) * a.D + c] = v;
+        }
+      }
+    }
+    if (tx == 0) {
+      if (!last) a.part_lse[(long long)blockIdx.z * a.tokens * a.Hq + at] = lse;
+      else if (a.lse != nullptr) a.lse[at] = lse;
+    }
+  }
+}
+
+// Joins the parts of one row (and the window's result): 128 threads, four columns each, groups of threads over the
+// parts, joined in a fixed order.
+template <typename T>
+__global__ void __launch_bounds__(128) prefix_join(const PrefixArgs a) {
+  extern __shared__ float smem[];       // weights [splits], then sums [groups][Dp]
+  const long long at = blockIdx.x, rows = a.tokens * a.Hq;
+  const int Dp = (a.D + 3) & ~3, cols = Dp / 4, groups = cols >= 128 ? 1 : 128 / cols;
+  float* w = smem;
+  float* acc = smem + ((a.splits + 3) & ~3);
+  __shared__ float red[4];
+  float m = a.window_lse != nullptr ? a.window_lse[at] : -INFINITY;
+  const float lw = m;
+  for (int i = threadIdx.x; i < a.splits; i += 128) {
+    w[i] = a.part_lse[(long long)i * rows + at];
+    m = fmaxf(m, w[i]);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const float base = m == -INFINITY ? 0.f : m;
+  float total = a.window_lse != nullptr ? expf(lw - base) : 0.f;
+  const float ww = total;
+  for (int i = 0; i < a.splits; ++i) total += expf(w[i] - base);
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+  const int g = threadIdx.x / cols, c = (threadIdx.x - g * cols) * 4;
+  if (g < groups && cols <= 128) {
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    const bool vec = a.D % 4 == 0;
+#pragma unroll 4
+    for (int i = g; i < a.splits; i += groups) {
+      const float e = expf(w[i] - base) * inv;
+      const float* p = a.part_out + ((long long)i * rows + at) * a.D + c;
+      if (vec) {
+        const float4 v = *reinterpret_cast<const float4*>(p);
+        if (e != 0.f) { s[0] = fmaf(e, v.x, s[0]); s[1] = fmaf(e, v.y, s[1]); s[2] = fmaf(e, v.z, s[2]); s[3] = fmaf(e, v.w, s[3]); }
+      } else if (e != 0.f) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          if (c + x < a.D) s[x] = fmaf(e, p[x], s[x]);
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < 4; ++x) acc[g * Dp + c + x] = s[x];
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < a.D; d += 128) {
+    float v = 0.f;
+    for (int i = 0; i < groups; ++i) v += acc[i * Dp + d];
+    if (a.window_lse != nullptr && ww != 0.f) v = fmaf(ww * inv, to_f<T>(static_cast<const T*>(a.window_out)[at * a.D + d]), v);
+    static_cast<T*>(a.out)[at * a.D + d] = from_f<T>(v);
+  }
+  if (threadIdx.x == 0 && a.lse != nullptr) a.lse[at] = m == -INFINITY ? m : m + logf(total);
+}
+
+int simt_bm(const PrefixArgs& a) { return a.tokens * a.G > 16 ? 64 : 16; }
+int simt_bn(const PrefixArgs& a) { return a.D <= 64 ? 64 : 32; }
+
+template <typename T, int BM, int BN, int NJ>
+int launch(const PrefixArgs& a, cudaStream_t s) {
+  const int Dp = (a.D + 3) & ~3;
+  const size_t smem = (size_t)(BM * (Dp + 4) + BN * (Dp + 4) + BN * Dp + BM * (BN + 4)) * sizeof(float);
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(prefix_simt<T, BM, BN, NJ>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) {
+      (void)cudaGetLastError();
+      return set_error(NATTEN_B200_ELAUNCH, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+    }
+  }
+  const long long rows = a.tokens * a.G;
+  const dim3 grid((unsigned)((rows + BM - 1) / BM), a.Hkv, a.splits);
+  // four elements at a time when every row starts on such a boundary
+  const uintptr_t all = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v |
+                        (uintptr_t)((a.q_token | a.q_head | a.k_token | a.k_head | a.v_token | a.v_head) * (long long)sizeof(T));
+  const bool vec = all % (4 * sizeof(T)) == 0;
+  NB_LAUNCH("prefix_simt", s, prefix_simt<T, BM, BN, NJ><<<grid, 256, smem, s>>>(a, vec));
+  return check_launch("prefix attention");
+}
+
+template <typename T>
+int run(const PrefixArgs& a, cudaStream_t s) {
+  const bool small = simt_bm(a) == 16;
+  if (a.D <= 64) return small ? launch<T, 16, 64, 1>(a, s) : launch<T, 64, 64, 1>(a, s);
+  if (a.D <= 128) return small ? launch<T, 16, 32, 2>(a, s) : launch<T, 64, 32, 2>(a, s);
+  return small ? launch<T, 16, 32, 4>(a, s) : launch<T, 64, 32, 4>(a, s);
+}
+
+template <typename T>
+int join(const PrefixArgs& a, cudaStream_t s) {
+  const int Dp = (a.D + 3) & ~3, cols = Dp / 4, groups = cols >= 128 ? 1 : 128 / cols;
+  const size_t smem = (size_t)(((a.splits + 3) & ~3) + groups * Dp) * sizeof(float);
+  NB_LAUNCH("prefix_join", s, prefix_join<T><<<(unsigned)(a.tokens * a.Hq), 128, smem, s>>>(a));
+  return check_launch("prefix attention, joining the parts");
+}
+
+}  // namespace
+
+// Parts of the prefix: enough blocks for two on every SM, none shorter than four tiles.
+int prefix_simt_splits(const PrefixArgs& a) {
+  const int bm = simt_bm(a), bn = simt_bn(a);
+  const long long blocks = ((a.tokens * a.G + bm - 1) / bm) * a.Hkv;
+  const long long want = blocks >= kSMs * 2 ? 1 : kSMs * 2 / blocks, most = (a.prefix + 4 * bn - 1) / (4 * bn);
+  const long long n = want < most ? want : most;
+  return n < 1 ? 1 : (int)n;
+}
+
+int run_prefix_simt(const PrefixArgs& a, int dtype, cudaStream_t s) {
+  if (dtype == NATTEN_B200_F32) return run<float>(a, s);
+  return dtype == NATTEN_B200_F16 ? run<__half>(a, s) : run<__nv_bfloat16>(a, s);
+}
+
+namespace {
+
+int make_args(const natten_b200_prefix_geom* g, PrefixArgs* a) {
+  if (g == nullptr) return set_error(NATTEN_B200_EINVAL, "prefix: geometry is null");
+  if (g->dtype < NATTEN_B200_F32 || g->dtype > NATTEN_B200_BF16) return set_error(NATTEN_B200_EINVAL, "prefix: unsupported dtype %d", g->dtype);
+  if (g->heads_q < 1 || g->heads_kv < 1 || g->head_dim < 1) return set_error(NATTEN_B200_EINVAL, "prefix: heads and head_dim must be positive");
+  if (g->head_dim > 256) return set_error(NATTEN_B200_EINVAL, "prefix: head_dim must be at most 256, got %d", g->head_dim);
+  if (g->heads_q % g->heads_kv != 0)
+    return set_error(NATTEN_B200_EINVAL, "prefix: heads_q (%d) must be divisible by heads_kv (%d)", g->heads_q, g->heads_kv);
+  if (g->heads_kv > 65535) return set_error(NATTEN_B200_EINVAL, "prefix: at most 65535 key/value heads");
+  if (g->batch < 0 || g->tokens < 0 || g->prefix < 0) return set_error(NATTEN_B200_EINVAL, "prefix: sizes must not be negative");
+  if (g->batch > 0x7fffffffLL || g->tokens > 0x7fffffffLL || g->batch * g->tokens > 0x7fffffffLL / g->heads_q)
+    return set_error(NATTEN_B200_EINVAL, "prefix: more than 2^31 rows");
+  if (g->prefix > 0x7fffffffLL - 1024) return set_error(NATTEN_B200_EINVAL, "prefix: more than 2^31 tokens");
+  if (!(g->scale > 0.f) || isinf(g->scale)) return set_error(NATTEN_B200_EINVAL, "prefix: scale must be positive and finite");
+  a->Hq = g->heads_q; a->Hkv = g->heads_kv; a->G = g->heads_q / g->heads_kv; a->D = g->head_dim;
+  a->tokens = g->batch * g->tokens;
+  a->per_sample = (uint32_t)(g->tokens > 0 ? g->tokens : 1);
+  a->prefix = (int)g->prefix;
+  a->scale = g->scale;
+  a->lens = g->lens;
+  // a stride over an axis of length one is never taken: the dense one keeps the checks on strides simple
+  a->q_head = a->Hq > 1 ? g->q_head_stride : a->D;
+  a->q_token = a->tokens > 1 ? g->q_token_stride : (long long)a->Hq * a->D;
+  a->k_head = a->Hkv > 1 ? g->k_head_stride : a->D;
+  a->k_token = a->prefix > 1 ? g->k_token_stride : (long long)a->Hkv * a->D;
+  a->v_head = a->Hkv > 1 ? g->v_head_stride : a->D;
+  a->v_token = a->prefix > 1 ? g->v_token_stride : (long long)a->Hkv * a->D;
+  a->splits = 1;
+  return NATTEN_B200_OK;
+}
+
+// The family that serves the call and the parts it cuts the prefix into.
+int choose(const natten_b200_prefix_geom* g, PrefixArgs* a, bool* tc) {
+  const char* why = prefix_sm100_unsupported(*a, g->dtype);
+  *tc = g->path != NATTEN_B200_PATH_SIMT && why == nullptr;
+  if (g->path == NATTEN_B200_PATH_TCGEN05 && !*tc)
+    return set_error(NATTEN_B200_EINVAL, "prefix: shape not supported by the tcgen05 kernels: %s", why);
+  a->splits = *tc ? prefix_sm100_splits(*a) : prefix_simt_splits(*a);
+  return NATTEN_B200_OK;
+}
+
+size_t scratch_bytes_of(const PrefixArgs& a) {
+  return a.splits <= 1 ? 0 : (size_t)a.splits * (size_t)a.tokens * a.Hq * ((size_t)a.D + 1) * sizeof(float);
+}
+
+}  // namespace
+}  // namespace nb
+
+using namespace nb;
+
+extern "C" {
+
+size_t natten_b200_prefix_scratch_bytes(const natten_b200_prefix_geom* g) {
+  PrefixArgs a{};
+  bool tc;
+  if (make_args(g, &a) || a.tokens == 0 || choose(g, &a, &tc)) return 0;
+  return scratch_bytes_of(a);
+}
+
+int natten_b200_prefix_forward(const natten_b200_prefix_geom* g, const void* q, const void* k, const void* v,
+                               const void* window_out, const float* window_lse, void* out, float* lse, void* scratch,
+                               size_t scratch_bytes, void* stream) {
+  PrefixArgs a{};
+  if (int rc = make_args(g, &a)) return rc;
+  if (a.tokens == 0) return NATTEN_B200_OK;
+  if (q == nullptr || out == nullptr || (a.prefix > 0 && (k == nullptr || v == nullptr)))
+    return set_error(NATTEN_B200_EINVAL, "prefix: null tensor");
+  if ((window_out == nullptr) != (window_lse == nullptr))
+    return set_error(NATTEN_B200_EINVAL, "prefix: window_out and window_lse must both be given or both be null");
+  for (const void* p : {q, k, v, (const void*)window_out, (const void*)out, (const void*)scratch})
+    if (((uintptr_t)p & 15) != 0) return set_error(NATTEN_B200_EINVAL, "prefix: tensor pointers must be 16-byte aligned");
+  bool tc;
+  if (int rc = choose(g, &a, &tc)) return rc;
+  const size_t need = scratch_bytes_of(a);
+  if (need > 0 && (scratch == nullptr || scratch_bytes < need))
+    return set_error(NATTEN_B200_ERESOURCE, "prefix: scratch has %zu bytes, needs %zu", scratch == nullptr ? (size_t)0 : scratch_bytes, need);
+  a.q = q; a.k = k; a.v = v; a.window_out = window_out; a.window_lse = window_lse; a.out = out; a.lse = lse;
+  a.part_out = static_cast<float*>(scratch);
+  a.part_lse = a.part_out == nullptr ? nullptr : a.part_out + (size_t)a.splits * a.tokens * a.Hq * a.D;
+  cudaStream_t s = (cudaStream_t)stream;
+  set_last_path(tc ? "tcgen05" : "simt");
+  if (int rc = tc ? run_prefix_sm100(a, g->dtype, s) : run_prefix_simt(a, g->dtype, s)) return rc;
+  if (a.splits == 1) return NATTEN_B200_OK;
+  if (g->dtype == NATTEN_B200_F32) return join<float>(a, s);
+  return g->dtype == NATTEN_B200_F16 ? join<__half>(a, s) : join<__nv_bfloat16>(a, s);
+}
+
+}  // extern "C"

@@ -75,7 +75,7 @@ constexpr uint32_t kPollLimit = 2048;  // probes before a wait on the critical p
 // aborting (this wait ran out, or another one did before).
 // The retry loop exists once per kernel (it is reached only when the first probe fails, and a
 // dozen inlined copies of it would only take room in the instruction cache).
-__device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+static __device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
   for (uint32_t it = 0; it < kSpinLimit; ++it) {
     if (mbar_try_wait(bar, parity)) return true;
     if ((it & 63u) == 63u && *abort_flag) return false;

@@ -310,6 +310,161 @@ def merge_backward(o0, l0, o1, l1, grad_out, grad_lse):
 
 
 # ---------------------------------------------------------------------------
+# around the attention: layer norm, rotary positions, attention to a shared prefix
+# ---------------------------------------------------------------------------
+
+class _On:
+    """``torch.cuda.device`` that costs nothing when the tensor's device is the current one already."""
+    __slots__ = ("guard",)
+
+    def __init__(self, device):
+        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _strides(shape, stride):
+    """The axes as few (size, stride) pairs, outermost first: axes of one step are joined, those of size 1 dropped."""
+    pairs = []
+    for n, st in zip(shape, stride):
+        if n == 1:
+            continue
+        if pairs and pairs[-1][1] == n * st:
+            pairs[-1] = (pairs[-1][0] * n, st)
+        else:
+            pairs.append((n, st))
+    return pairs
+
+
+def _norm_rows(x):
+    """(x, natten_b200_rows): x itself when its rows follow one or two strides, else a dense copy."""
+    c = x.shape[-1]
+    rows = x.numel() // c
+    if x.is_contiguous():
+        return x, _lib.Rows(rows, 1, c, 0, c, 0)
+    pairs = _strides(x.shape[:-1], x.stride()[:-1]) if x.stride(-1) == 1 or c == 1 else None
+    if pairs is None or len(pairs) > 2:
+        x = x.contiguous()
+        return x, _lib.Rows(rows, 1, c, 0, c, 0)
+    if len(pairs) < 2:
+        return x, _lib.Rows(rows, 1, pairs[0][1] if pairs else c, 0, c, 0)
+    return x, _lib.Rows(rows, pairs[1][0], pairs[0][1], pairs[1][1], c, 0)
+
+
+def _weight_code(x, weight, bias):
+    w = weight if weight is not None else bias
+    return _DTYPES[x.dtype if w is None else w.dtype]
+
+
+def layer_norm_forward(x, weight, bias, eps, save=False):
+    """Returns (y, mean, rstd); the statistics are float32 over the rows, None without ``save``."""
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    mean = rstd = None
+    if save:
+        mean, rstd = torch.empty((2,) + tuple(x.shape[:-1]), dtype=torch.float32, device=x.device).unbind(0)
+    if y.numel():
+        x, rows = _norm_rows(x)
+        with _On(x.device):
+            _lib.check(_lib.load().natten_b200_layer_norm_forward(
+                _DTYPES[x.dtype], _weight_code(x, weight, bias), rows, x.data_ptr(), _ptr(weight), _ptr(bias), eps,
+                y.data_ptr(), _ptr(mean), _ptr(rstd), _stream(x)))
+    return y, mean, rstd
+
+
+def layer_norm_backward(x, weight, bias, mean, rstd, grad, want_dx, want_dw, want_db):
+    """Returns (dx, dweight, dbias), None for those that are not wanted."""
+    c = x.shape[-1]
+    like = weight if weight is not None else bias
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_dx else None
+    dw = torch.empty(c, dtype=like.dtype, device=x.device) if want_dw else None
+    db = torch.empty(c, dtype=like.dtype, device=x.device) if want_db else None
+    x, rows = _norm_rows(x)
+    grad = grad.contiguous()
+    lib = _lib.load()
+    nbytes = int(lib.natten_b200_layer_norm_backward_scratch_bytes(rows.rows, c)) if want_dw or want_db else 0
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+    with _On(x.device):
+        _lib.check(lib.natten_b200_layer_norm_backward(
+            _DTYPES[x.dtype], _weight_code(x, weight, bias), rows, _ptr(x), _ptr(weight), _ptr(mean), _ptr(rstd),
+            _ptr(grad), _ptr(dx), _ptr(dw), _ptr(db), _ptr(scratch), nbytes, _stream(x)))
+    return dx, dw, db
+
+
+def _token_head_strides(t):
+    """(t, token stride, head stride) of ``[..., heads, D]``: t itself when one stride leads through its tokens."""
+    heads, d = t.shape[-2:]
+    if not t.is_contiguous():
+        pairs = _strides(t.shape[:-2], t.stride()[:-2]) if t.stride(-1) == 1 or d == 1 else None
+        if pairs is not None and len(pairs) < 2:
+            return t, pairs[0][1] if pairs else heads * d, t.stride(-2) if heads > 1 else d
+        t = t.contiguous()
+    return t, heads * d, d
+
+
+def rotary(q, k, spec, origin, offsets, positions, inverse=False):
+    """Turns q and k; ``spec`` = (axis_dims, phases as a ctypes array, interleaved)."""
+    axis_dims, phases, interleaved = spec
+    yq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    yk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    if not q.numel():
+        return yq, yk
+    q, qt, qh = _token_head_strides(q)
+    k, kt, kh = _token_head_strides(k)
+    rank = q.dim() - 3
+    pad = (0,) * (3 - rank)
+    pos = positions if positions is not None else offsets
+    kind = _lib.POS_GRID if pos is None else _lib.POS_OFFSET if positions is None else _lib.POS_GIVEN
+    g = _lib.RotaryGeom(
+        _DTYPES[q.dtype], rank, q.shape[0], _lib._I3(*q.shape[1:-2], *pad), q.shape[-2], k.shape[-2], q.shape[-1],
+        len(axis_dims), _lib._I3(*axis_dims), qt, qh, kt, kh, interleaved, kind,
+        64 if pos is not None and pos.dtype == torch.int64 else 32, positions is not None and positions.shape[0] == q.shape[0],
+        (ctypes.c_int64 * 3)(*origin), _ptr(pos), ctypes.addressof(phases))
+    with _On(q.device):
+        _lib.check(_lib.load().natten_b200_rotary(g, q.data_ptr(), k.data_ptr(), yq.data_ptr(), yk.data_ptr(),
+                                                  1 if inverse else 0, _stream(q)))
+    return yq, yk
+
+
+def _tma_strides(t, d):
+    """As _token_head_strides, but a dense copy unless the strides and the address are multiples of 16 bytes."""
+    t, token, head = _token_head_strides(t)
+    step = 16 // t.element_size()
+    if t.data_ptr() % 16 or token < 1 or head < 1 or (not t.is_contiguous() and (token % step or head % step)):
+        t = t.clone(memory_format=torch.contiguous_format)
+        token, head = t.shape[-2] * d, d
+    return t, token, head
+
+
+def prefix_forward(q, k, v, scale, lens=None, window_out=None, window_lse=None, path=None):
+    """Returns (out, lse) of the queries over the shared prefix (and the window's keys)."""
+    d = q.shape[-1]
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device)
+    if not out.numel():
+        return out, lse
+    q, qt, qh = _tma_strides(q, d)
+    k, kt, kh = _tma_strides(k, d)
+    v, vt, vh = _tma_strides(v, d)
+    if window_out is not None:
+        window_out, = _prep(window_out)
+    g = _lib.PrefixGeom(_DTYPES[q.dtype], q.shape[-2], k.shape[-2], d, q.shape[0], q[0, ..., 0, 0].numel(), k.shape[0],
+                        qt, qh, kt, kh, vt, vh, _scale(scale, d), _PATHS[_fused_path if path is None else path], _ptr(lens))
+    lib = _lib.load()
+    nbytes = int(lib.natten_b200_prefix_scratch_bytes(g))
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    with _On(q.device):
+        _lib.check(lib.natten_b200_prefix_forward(g, _ptr(q), _ptr(k), _ptr(v), _ptr(window_out), _ptr(window_lse),
+                                                  _ptr(out), _ptr(lse), _ptr(scratch), nbytes, _stream(q)))
+    return out, lse
+
+
+# ---------------------------------------------------------------------------
 # the backend-module protocol (names and argument order of the reference)
 # ---------------------------------------------------------------------------
 

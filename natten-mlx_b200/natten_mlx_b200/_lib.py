@@ -51,8 +51,34 @@ class Geom(ctypes.Structure):
     ]
 
 
+class Rows(ctypes.Structure):
+    """Mirrors natten_b200_rows."""
+    _fields_ = [("rows", ctypes.c_int64), ("inner", ctypes.c_int64), ("outer_stride", ctypes.c_int64),
+                ("inner_stride", ctypes.c_int64), ("channels", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class RotaryGeom(ctypes.Structure):
+    """Mirrors natten_b200_rotary_geom."""
+    _fields_ = ([("dtype", ctypes.c_int32), ("rank", ctypes.c_int32), ("batch", ctypes.c_int64), ("extent", _I3)] +
+                [(n, ctypes.c_int32) for n in ("heads_q", "heads_k", "head_dim", "n_axes")] + [("axis_dims", _I3)] +
+                [(n, ctypes.c_int64) for n in ("q_token_stride", "q_head_stride", "k_token_stride", "k_head_stride")] +
+                [(n, ctypes.c_int32) for n in ("interleaved", "position_kind", "position_bits", "position_batch")] +
+                [("origin", ctypes.c_int64 * 3), ("positions", ctypes.c_void_p), ("phases", ctypes.c_void_p)])
+
+
+class PrefixGeom(ctypes.Structure):
+    """Mirrors natten_b200_prefix_geom."""
+    _fields_ = ([(n, ctypes.c_int32) for n in ("dtype", "heads_q", "heads_kv", "head_dim")] +
+                [(n, ctypes.c_int64) for n in ("batch", "tokens", "prefix", "q_token_stride", "q_head_stride",
+                                               "k_token_stride", "k_head_stride", "v_token_stride", "v_head_stride")] +
+                [("scale", ctypes.c_float), ("path", ctypes.c_int32), ("lens", ctypes.c_void_p)])
+
+
+POS_GRID, POS_OFFSET, POS_GIVEN = 0, 1, 2
+
 _P = ctypes.c_void_p
 _G = ctypes.POINTER(Geom)
+_I32 = ctypes.c_int32
 
 # name -> (restype, argtypes); every symbol the header declares.
 SYMBOLS = {
@@ -82,6 +108,12 @@ SYMBOLS = {
     "natten_b200_plan_hint": (ctypes.c_int, [_G, ctypes.c_int32, _P, ctypes.c_int32]),
     "natten_b200_merge_forward": (ctypes.c_int, [ctypes.c_int32, ctypes.c_int64, ctypes.c_int32] + [_P] * 7),
     "natten_b200_merge_backward": (ctypes.c_int, [ctypes.c_int32, ctypes.c_int64, ctypes.c_int32] + [_P] * 11),
+    "natten_b200_layer_norm_forward": (ctypes.c_int, [_I32, _I32, ctypes.POINTER(Rows), _P, _P, _P, ctypes.c_float] + [_P] * 4),
+    "natten_b200_layer_norm_backward_scratch_bytes": (ctypes.c_size_t, [ctypes.c_int64, _I32]),
+    "natten_b200_layer_norm_backward": (ctypes.c_int, [_I32, _I32, ctypes.POINTER(Rows)] + [_P] * 9 + [ctypes.c_size_t, _P]),
+    "natten_b200_rotary": (ctypes.c_int, [ctypes.POINTER(RotaryGeom)] + [_P] * 4 + [_I32, _P]),
+    "natten_b200_prefix_scratch_bytes": (ctypes.c_size_t, [ctypes.POINTER(PrefixGeom)]),
+    "natten_b200_prefix_forward": (ctypes.c_int, [ctypes.POINTER(PrefixGeom)] + [_P] * 8 + [ctypes.c_size_t, _P]),
 }
 
 class HaloOut(ctypes.Structure):
