@@ -311,22 +311,17 @@ def merge_backward(o0, l0, o1, l1, grad_out, grad_lse):
 
 # ---------------------------------------------------------------------------
 # around the attention: layer norm, rotary positions, attention to a shared prefix
+#
+# These take a few microseconds on the device in serving, so the host side is kept short: no context manager while the
+# tensor's device is the current one, the raw stream handle, one allocation where two would do.
 # ---------------------------------------------------------------------------
 
-class _On:
-    """``torch.cuda.device`` that costs nothing when the tensor's device is the current one already."""
-    __slots__ = ("guard",)
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch.cuda.current_device
 
-    def __init__(self, device):
-        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _elsewhere(device) -> bool:
+    return device.index != _current_device()
 
 
 def _strides(shape, stride):
@@ -345,54 +340,66 @@ def _strides(shape, stride):
 def _norm_rows(x):
     """(x, natten_b200_rows): x itself when its rows follow one or two strides, else a dense copy."""
     c = x.shape[-1]
-    rows = x.numel() // c
-    if x.is_contiguous():
-        return x, _lib.Rows(rows, 1, c, 0, c, 0)
-    pairs = _strides(x.shape[:-1], x.stride()[:-1]) if x.stride(-1) == 1 or c == 1 else None
-    if pairs is None or len(pairs) > 2:
+    if not x.is_contiguous():
+        pairs = _strides(x.shape[:-1], x.stride()[:-1]) if x.stride(-1) == 1 or c == 1 else ()
+        if len(pairs) == 1:
+            return x, _lib.Rows(x.numel() // c, 1, pairs[0][1], 0, c, 0)
+        if len(pairs) == 2:
+            return x, _lib.Rows(x.numel() // c, pairs[1][0], pairs[0][1], pairs[1][1], c, 0)
         x = x.contiguous()
-        return x, _lib.Rows(rows, 1, c, 0, c, 0)
-    if len(pairs) < 2:
-        return x, _lib.Rows(rows, 1, pairs[0][1] if pairs else c, 0, c, 0)
-    return x, _lib.Rows(rows, pairs[1][0], pairs[0][1], pairs[1][1], c, 0)
+    return x, _lib.Rows(x.numel() // c, 1, c, 0, c, 0)
 
 
-def _weight_code(x, weight, bias):
-    w = weight if weight is not None else bias
-    return _DTYPES[x.dtype if w is None else w.dtype]
+def _dense_like(x):
+    return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
 
 
 def layer_norm_forward(x, weight, bias, eps, save=False):
-    """Returns (y, mean, rstd); the statistics are float32 over the rows, None without ``save``."""
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean = rstd = None
-    if save:
-        mean, rstd = torch.empty((2,) + tuple(x.shape[:-1]), dtype=torch.float32, device=x.device).unbind(0)
-    if y.numel():
-        x, rows = _norm_rows(x)
-        with _On(x.device):
-            _lib.check(_lib.load().natten_b200_layer_norm_forward(
-                _DTYPES[x.dtype], _weight_code(x, weight, bias), rows, x.data_ptr(), _ptr(weight), _ptr(bias), eps,
-                y.data_ptr(), _ptr(mean), _ptr(rstd), _stream(x)))
-    return y, mean, rstd
-
-
-def layer_norm_backward(x, weight, bias, mean, rstd, grad, want_dx, want_dw, want_db):
-    """Returns (dx, dweight, dbias), None for those that are not wanted."""
-    c = x.shape[-1]
-    like = weight if weight is not None else bias
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_dx else None
-    dw = torch.empty(c, dtype=like.dtype, device=x.device) if want_dw else None
-    db = torch.empty(c, dtype=like.dtype, device=x.device) if want_db else None
+    """Returns (y, stats): the means and then the reciprocal deviations of the rows, float32 ``[2, rows]``, or None
+    without ``save``."""
+    device = x.device
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return layer_norm_forward(x, weight, bias, eps, save)
+    y = _dense_like(x)
     x, rows = _norm_rows(x)
-    grad = grad.contiguous()
+    n = rows.rows
+    stats = torch.empty((2, n), dtype=torch.float32, device=device) if save else None
+    if n:
+        like = weight if weight is not None else bias if bias is not None else x
+        mean = 0 if stats is None else stats.data_ptr()
+        rc = _lib.load().natten_b200_layer_norm_forward(
+            _DTYPES[x.dtype], _DTYPES[like.dtype], rows, x.data_ptr(), _ptr(weight), _ptr(bias), eps, y.data_ptr(),
+            mean, mean and mean + 4 * n, _raw_stream(device.index))
+        if rc:
+            _lib.check(rc)
+    return y, stats
+
+
+def layer_norm_backward(x, weight, bias, stats, grad, want_dx, want_dw, want_db):
+    """Returns (dx, dweight, dbias), None for those that are not wanted."""
+    device = x.device
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return layer_norm_backward(x, weight, bias, stats, grad, want_dx, want_dw, want_db)
+    like = weight if weight is not None else bias if bias is not None else x
+    dx = _dense_like(x) if want_dx else None
+    dw = torch.empty_like(weight) if want_dw else None
+    db = torch.empty_like(bias) if want_db else None
+    x, rows = _norm_rows(x)
+    if not grad.is_contiguous():
+        grad = grad.contiguous()
     lib = _lib.load()
-    nbytes = int(lib.natten_b200_layer_norm_backward_scratch_bytes(rows.rows, c)) if want_dw or want_db else 0
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
-    with _On(x.device):
-        _lib.check(lib.natten_b200_layer_norm_backward(
-            _DTYPES[x.dtype], _weight_code(x, weight, bias), rows, _ptr(x), _ptr(weight), _ptr(mean), _ptr(rstd),
-            _ptr(grad), _ptr(dx), _ptr(dw), _ptr(db), _ptr(scratch), nbytes, _stream(x)))
+    n, nbytes, scratch = rows.rows, 0, None
+    if want_dw or want_db:
+        nbytes = lib.natten_b200_layer_norm_backward_scratch_bytes(n, rows.channels)
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    mean = stats.data_ptr()
+    rc = lib.natten_b200_layer_norm_backward(
+        _DTYPES[x.dtype], _DTYPES[like.dtype], rows, x.data_ptr(), _ptr(weight), mean, mean + 4 * n, grad.data_ptr(),
+        _ptr(dx), _ptr(dw), _ptr(db), _ptr(scratch), nbytes, _raw_stream(device.index))
+    if rc:
+        _lib.check(rc)
     return dx, dw, db
 
 
@@ -407,27 +414,31 @@ def _token_head_strides(t):
     return t, heads * d, d
 
 
-def rotary(q, k, spec, origin, offsets, positions, inverse=False):
-    """Turns q and k; ``spec`` = (axis_dims, phases as a ctypes array, interleaved)."""
-    axis_dims, phases, interleaved = spec
-    yq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    yk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    if not q.numel():
+def rotary(q, k, spec, origin, offsets, positions, inverse=0):
+    """Turns q and k; ``spec`` = (axes, axis_dims as three int32, phases as uint64, interleaved), ``origin`` three int64."""
+    device = q.device
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return rotary(q, k, spec, origin, offsets, positions, inverse)
+    yq, yk = _dense_like(q), _dense_like(k)
+    if not yq.numel():
         return yq, yk
     q, qt, qh = _token_head_strides(q)
     k, kt, kh = _token_head_strides(k)
-    rank = q.dim() - 3
-    pad = (0,) * (3 - rank)
-    pos = positions if positions is not None else offsets
-    kind = _lib.POS_GRID if pos is None else _lib.POS_OFFSET if positions is None else _lib.POS_GIVEN
-    g = _lib.RotaryGeom(
-        _DTYPES[q.dtype], rank, q.shape[0], _lib._I3(*q.shape[1:-2], *pad), q.shape[-2], k.shape[-2], q.shape[-1],
-        len(axis_dims), _lib._I3(*axis_dims), qt, qh, kt, kh, interleaved, kind,
-        64 if pos is not None and pos.dtype == torch.int64 else 32, positions is not None and positions.shape[0] == q.shape[0],
-        (ctypes.c_int64 * 3)(*origin), _ptr(pos), ctypes.addressof(phases))
-    with _On(q.device):
-        _lib.check(_lib.load().natten_b200_rotary(g, q.data_ptr(), k.data_ptr(), yq.data_ptr(), yk.data_ptr(),
-                                                  1 if inverse else 0, _stream(q)))
+    shape = q.shape
+    rank = len(shape) - 3
+    pos, kind = (positions, _lib.POS_GIVEN) if positions is not None else (offsets, _lib.POS_OFFSET)
+    if pos is None:
+        bits, batch, kind, where = 32, 0, _lib.POS_GRID, None
+    else:
+        bits, batch, where = 64 if pos.dtype == torch.int64 else 32, pos.shape[0] == shape[0], pos.data_ptr()
+    axes, axis_dims, phases, interleaved = spec
+    g = _lib.RotaryGeom(_DTYPES[q.dtype], rank, shape[0], (shape[1:-2] + (0, 0))[:3], shape[-2], k.shape[-2], shape[-1], axes,
+                        axis_dims, qt, qh, kt, kh, interleaved, kind, bits, batch, origin, where, ctypes.addressof(phases))
+    rc = _lib.load().natten_b200_rotary(g, q.data_ptr(), k.data_ptr(), yq.data_ptr(), yk.data_ptr(), inverse,
+                                        _raw_stream(device.index))
+    if rc:
+        _lib.check(rc)
     return yq, yk
 
 
@@ -443,9 +454,13 @@ def _tma_strides(t, d):
 
 def prefix_forward(q, k, v, scale, lens=None, window_out=None, window_lse=None, path=None):
     """Returns (out, lse) of the queries over the shared prefix (and the window's keys)."""
+    device = q.device
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return prefix_forward(q, k, v, scale, lens, window_out, window_lse, path)
     d = q.shape[-1]
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device)
+    out = _dense_like(q)
+    lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=device)
     if not out.numel():
         return out, lse
     q, qt, qh = _tma_strides(q, d)
@@ -453,14 +468,16 @@ def prefix_forward(q, k, v, scale, lens=None, window_out=None, window_lse=None, 
     v, vt, vh = _tma_strides(v, d)
     if window_out is not None:
         window_out, = _prep(window_out)
-    g = _lib.PrefixGeom(_DTYPES[q.dtype], q.shape[-2], k.shape[-2], d, q.shape[0], q[0, ..., 0, 0].numel(), k.shape[0],
+    batch, heads = q.shape[0], q.shape[-2]
+    g = _lib.PrefixGeom(_DTYPES[q.dtype], heads, k.shape[-2], d, batch, q.numel() // (batch * heads * d), k.shape[0],
                         qt, qh, kt, kh, vt, vh, _scale(scale, d), _PATHS[_fused_path if path is None else path], _ptr(lens))
     lib = _lib.load()
-    nbytes = int(lib.natten_b200_prefix_scratch_bytes(g))
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    with _On(q.device):
-        _lib.check(lib.natten_b200_prefix_forward(g, _ptr(q), _ptr(k), _ptr(v), _ptr(window_out), _ptr(window_lse),
-                                                  _ptr(out), _ptr(lse), _ptr(scratch), nbytes, _stream(q)))
+    nbytes = lib.natten_b200_prefix_scratch_bytes(g)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    rc = lib.natten_b200_prefix_forward(g, q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(window_out), _ptr(window_lse),
+                                        out.data_ptr(), lse.data_ptr(), _ptr(scratch), nbytes, _raw_stream(device.index))
+    if rc:
+        _lib.check(rc)
     return out, lse
 
 

@@ -109,19 +109,28 @@ class _Merge(torch.autograd.Function):
         return do0, dl0.to(l0.dtype), do1, dl1.to(l1.dtype)
 
 
+def _once(backward):
+    """A backward that cannot be differentiated itself.  Only a pass that builds a graph (``create_graph=True``) pays for
+    the wrapper that says so when that graph is used."""
+    guarded = once_differentiable(backward)
+
+    def call(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return call
+
+
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, mean, rstd = _cuda.layer_norm_forward(x, weight, bias, eps, save=True)
-        ctx.save_for_backward(x, weight, bias, mean, rstd)
+        y, stats = _cuda.layer_norm_forward(x, weight, bias, eps, True)
+        ctx.save_for_backward(x, weight, bias, stats)
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad):
-        x, weight, bias, mean, rstd = ctx.saved_tensors
         need = ctx.needs_input_grad
-        return _cuda.layer_norm_backward(x, weight, bias, mean, rstd, grad, need[0], need[1], need[2]) + (None,)
+        return (*_cuda.layer_norm_backward(*ctx.saved_tensors, grad, need[0], need[1], need[2]), None)
 
 
 class _Rotary(torch.autograd.Function):
@@ -134,12 +143,9 @@ class _Rotary(torch.autograd.Function):
         return _cuda.rotary(q, k, spec, origin, offsets, positions)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad_q, grad_k):
-        offsets, positions = ctx.saved_tensors
-        spec, origin = ctx.params
-        dq, dk = _cuda.rotary(grad_q, grad_k, spec, origin, offsets, positions, inverse=True)
-        return dq, dk, None, None, None, None
+        return (*_cuda.rotary(grad_q, grad_k, *ctx.params, *ctx.saved_tensors, 1), None, None, None, None)
 
 
 def layer_norm_with_grad(x, weight, bias, eps):

@@ -21,6 +21,7 @@ from ._core import cuda as _cuda
 from .utils.params import normalize_tuple_param
 
 _TWO_PI = Decimal("6.28318530717958647692528676655900576839433879875021164194988918461563281257241799725606965068")
+_NO_ORIGIN = (ctypes.c_int64 * 3)()
 _LAYOUTS = {1: "[B, L, heads, dim]", 2: "[B, H, W, heads, dim]", 3: "[B, D, H, W, heads, dim]"}
 
 
@@ -45,7 +46,9 @@ def _phases(axis_dims: Tuple[int, ...], base: float, frequencies: Optional[Tuple
 
 @lru_cache(maxsize=128)
 def _spec(axis_dims: Tuple[int, ...], base: float, frequencies: Optional[Tuple[float, ...]], interleaved: bool):
-    return axis_dims, _phases(axis_dims, base, frequencies), interleaved
+    """What a call hands to the library, once for each choice of arguments."""
+    dims = (ctypes.c_int32 * 3)(*axis_dims, *(0,) * (3 - len(axis_dims)))
+    return len(axis_dims), dims, _phases(axis_dims, base, frequencies), int(interleaved)
 
 
 def _check_positions(name, t, shape_ok, expected, query):
@@ -105,7 +108,7 @@ def rotary(query: torch.Tensor, key: torch.Tensor, axis_dims: Optional[Sequence[
         frequencies = tuple(float(f) for f in frequencies)
         if len(frequencies) != sum(dims) // 2 or not all(math.isfinite(f) for f in frequencies):
             raise ValueError(f"frequencies must be {sum(dims) // 2} finite numbers, got {len(frequencies)}")
-    origin, start = (0, 0, 0), None
+    origin, start = _NO_ORIGIN, None
     if positions is not None:
         if offsets is not None:
             raise ValueError("offsets and positions cannot be combined")
@@ -123,7 +126,7 @@ def rotary(query: torch.Tensor, key: torch.Tensor, axis_dims: Optional[Sequence[
             given = normalize_tuple_param(offsets, rank, "offsets")
             if not all(isinstance(o, int) and -2 ** 62 < o < 2 ** 62 for o in given):
                 raise ValueError(f"offsets must be integers, got {offsets!r}")
-            origin = tuple(given) + (0,) * (3 - rank)
+            origin = (ctypes.c_int64 * 3)(*given, *(0,) * (3 - rank))
     spec = _spec(dims, base, frequencies, bool(interleaved))
     if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad):
         return _ag.rotary_with_grad(query, key, spec, origin, start, positions)
