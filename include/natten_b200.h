@@ -414,7 +414,7 @@ int natten_b200_rotary(const natten_b200_rotary_geom* g, const void* q, const vo
  * first lens[b] tokens only; a row that sees none gets out 0 and lse -inf, and nothing that k or v hold past a sample's
  * length reaches its rows.  With window_out / window_lse (both or neither: the same queries' result over other keys,
  * such as natten_b200_fused_forward leaves) out and lse are those of the union of both sets of keys, as
- * natten_b200_merge_forward would join them.  scratch: natten_b200_prefix_scratch_bytes, 16-byte aligned, may be null
+ * natten_b200_merge_forward would join them.  scratch: natten_b200_prefix_scratch_bytes, 32-byte aligned, may be null
  * when that is 0.  Forward only.  bf16 / fp16 with head_dim a multiple of 8 up to 128 run on the tensor cores, the rest
  * (head_dim up to 256) on the CUDA cores; path as in the fused entry points.  The extra tokens of the fused entry points
  * belong to one sample each; the reference's composition for them is src/natten_mlx/functional.py:71-104.

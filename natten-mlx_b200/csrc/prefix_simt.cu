@@ -9,6 +9,8 @@
 // reading of k and v, which then is spread over all SMs by splitting the prefix.
 #include <math.h>
 
+#include <algorithm>
+
 #include "prefix.cuh"
 
 namespace nb {
@@ -43,6 +45,7 @@ __device__ __forceinline__ float4 load4(const T* row, int c, int D, bool vec, bo
 template <typename T, int BM, int BN, int NJ>
 __global__ void __launch_bounds__(256) prefix_simt(const PrefixArgs a, bool vec) {
   constexpr int RM = BM / 16, CN = BN / 16;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");     // the joining kernel may be set up meanwhile
   extern __shared__ float smem[];
   const int Dp = (a.D + 3) & ~3, LD = Dp + 4;
   float* qs = smem;                    // [BM][LD]
@@ -219,60 +222,91 @@ __global__ void __launch_bounds__(256) prefix_simt(const PrefixArgs a, bool vec)
   }
 }
 
-// Joins the parts of one row (and the window's result): 128 threads, four columns each, groups of threads over the
-// parts, joined in a fixed order.
-template <typename T>
-__global__ void __launch_bounds__(128) prefix_join(const PrefixArgs a) {
-  extern __shared__ float smem[];       // weights [splits], then sums [groups][Dp]
-  const long long at = blockIdx.x, rows = a.tokens * a.Hq;
-  const int Dp = (a.D + 3) & ~3, cols = Dp / 4, groups = cols >= 128 ? 1 : 128 / cols;
-  float* w = smem;
-  float* acc = smem + ((a.splits + 3) & ~3);
-  __shared__ float red[4];
-  float m = a.window_lse != nullptr ? a.window_lse[at] : -INFINITY;
-  const float lw = m;
-  for (int i = threadIdx.x; i < a.splits; i += 128) {
-    w[i] = a.part_lse[(long long)i * rows + at];
-    m = fmaxf(m, w[i]);
-  }
+// Joins the parts of a row and the window's result: 4 columns per lane, and where a row leaves lanes over they take other
+// parts; WARPS warps share a row's parts.  The order of the sums is fixed.  The kernel starts while the one that writes
+// the parts still runs, and waits for its end.
+constexpr int kMostParts = 256;
+
+template <typename T, int WARPS>
+__global__ void __launch_bounds__(128) prefix_join(const PrefixArgs a, int lanes) {
+  __shared__ float weight[4 / WARPS][WARPS == 1 ? 8 : kMostParts];
+  __shared__ float4 sums[WARPS][64];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, of = warp % WARPS, slot = warp / WARPS;
+  const long long part = (long long)blockIdx.x * (4 / WARPS) + slot, rows = a.part_rows;
+  const long long at = part < rows ? prefix_part_row(a, part) : -1;      // one row for all warps that meet below
+  if (at < 0) return;
+  const float lw = a.window_lse != nullptr ? a.window_lse[at] : -INFINITY;
+  float m = lw;
+  for (int i = lane; i < a.splits; i += 32) m = fmaxf(m, a.part_lse[i * rows + part]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
   const float base = m == -INFINITY ? 0.f : m;
-  float total = a.window_lse != nullptr ? expf(lw - base) : 0.f;
-  const float ww = total;
-  for (int i = 0; i < a.splits; ++i) total += expf(w[i] - base);
-  const float inv = total == 0.f ? 0.f : 1.f / total;
-  const int g = threadIdx.x / cols, c = (threadIdx.x - g * cols) * 4;
-  if (g < groups && cols <= 128) {
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
-    const bool vec = a.D % 4 == 0;
-#pragma unroll 4
-    for (int i = g; i < a.splits; i += groups) {
-      const float e = expf(w[i] - base) * inv;
-      const float* p = a.part_out + ((long long)i * rows + at) * a.D + c;
-      if (vec) {
-        const float4 v = *reinterpret_cast<const float4*>(p);
-        if (e != 0.f) { s[0] = fmaf(e, v.x, s[0]); s[1] = fmaf(e, v.y, s[1]); s[2] = fmaf(e, v.z, s[2]); s[3] = fmaf(e, v.w, s[3]); }
-      } else if (e != 0.f) {
+  float total = 0.f;
+  for (int i = lane; i < a.splits; i += 32) {
+    const float e = expf(a.part_lse[i * rows + part] - base);
+    weight[slot][i] = e;                                   // the warps of a row write the same
+    total += e;
+  }
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
-          if (c + x < a.D) s[x] = fmaf(e, p[x], s[x]);
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  const float ww = a.window_lse != nullptr ? expf(lw - base) : 0.f;
+  total += ww;
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+  __syncwarp();
+  const int groups = 32 / lanes * WARPS, group = of * (32 / lanes) + lane / lanes;
+  const int cols = (a.D + 3) / 4;
+  const bool vec = a.D % 4 == 0;
+  for (int first = 0; first < cols; first += lanes) {      // once, twice for head dims above 128
+    const int c4 = first + lane % lanes;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (c4 < cols) {
+#pragma unroll 8
+      for (int i = group; i < a.splits; i += groups) {
+        const float e = weight[slot][i];                   // 0 for a part without keys, which left zeros
+        const float* p = a.part_out + (i * rows + part) * a.D + c4 * 4;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (vec) {
+          v = __ldg(reinterpret_cast<const float4*>(p));
+        } else {
+          v.x = p[0];
+          if (c4 * 4 + 1 < a.D) v.y = p[1];
+          if (c4 * 4 + 2 < a.D) v.z = p[2];
+          if (c4 * 4 + 3 < a.D) v.w = p[3];
+        }
+        s.x = fmaf(e, v.x, s.x); s.y = fmaf(e, v.y, s.y); s.z = fmaf(e, v.z, s.z); s.w = fmaf(e, v.w, s.w);
       }
     }
+    for (int o = 16; o >= lanes; o >>= 1) {
+      s.x += __shfl_xor_sync(0xffffffffu, s.x, o); s.y += __shfl_xor_sync(0xffffffffu, s.y, o);
+      s.z += __shfl_xor_sync(0xffffffffu, s.z, o); s.w += __shfl_xor_sync(0xffffffffu, s.w, o);
+    }
+    if (WARPS > 1) {
+      if (lane < lanes) sums[of][c4] = s;
+    } else if (lane < lanes && c4 < cols) {
+      const float v[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
-    for (int x = 0; x < 4; ++x) acc[g * Dp + c + x] = s[x];
+      for (int x = 0; x < 4; ++x)
+        if (c4 * 4 + x < a.D) {
+          float o = v[x] * inv;
+          if (ww != 0.f) o = fmaf(ww * inv, to_f<T>(static_cast<const T*>(a.window_out)[at * a.D + c4 * 4 + x]), o);
+          static_cast<T*>(a.out)[at * a.D + c4 * 4 + x] = from_f<T>(o);
+        }
+    }
   }
-  __syncthreads();
-  for (int d = threadIdx.x; d < a.D; d += 128) {
-    float v = 0.f;
-    for (int i = 0; i < groups; ++i) v += acc[i * Dp + d];
-    if (a.window_lse != nullptr && ww != 0.f) v = fmaf(ww * inv, to_f<T>(static_cast<const T*>(a.window_out)[at * a.D + d]), v);
-    static_cast<T*>(a.out)[at * a.D + d] = from_f<T>(v);
+  if (WARPS > 1) {
+    __syncthreads();
+    const float* s = reinterpret_cast<const float*>(sums);
+    for (int d = threadIdx.x; d < a.D; d += 128) {
+      float o = 0.f;
+#pragma unroll
+      for (int i = 0; i < WARPS; ++i) o += s[i * 256 + d];
+      o *= inv;
+      if (ww != 0.f) o = fmaf(ww * inv, to_f<T>(static_cast<const T*>(a.window_out)[at * a.D + d]), o);
+      static_cast<T*>(a.out)[at * a.D + d] = from_f<T>(o);
+    }
   }
-  if (threadIdx.x == 0 && a.lse != nullptr) a.lse[at] = m == -INFINITY ? m : m + logf(total);
+  if (of == 0 && lane == 0 && a.lse != nullptr) a.lse[at] = m == -INFINITY ? m : m + logf(total);
 }
 
 int simt_bm(const PrefixArgs& a) { return a.tokens * a.G > 16 ? 64 : 16; }
@@ -309,9 +343,25 @@ int run(const PrefixArgs& a, cudaStream_t s) {
 
 template <typename T>
 int join(const PrefixArgs& a, cudaStream_t s) {
-  const int Dp = (a.D + 3) & ~3, cols = Dp / 4, groups = cols >= 128 ? 1 : 128 / cols;
-  const size_t smem = (size_t)(((a.splits + 3) & ~3) + groups * Dp) * sizeof(float);
-  NB_LAUNCH("prefix_join", s, prefix_join<T><<<(unsigned)(a.tokens * a.Hq), 128, smem, s>>>(a));
+  int lanes = 1;                         // of a row: a power of two
+  while (lanes < 32 && lanes * 4 < a.D) lanes *= 2;
+  cudaLaunchConfig_t cfg{};
+  cfg.blockDim = dim3(128);
+  cfg.stream = s;
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  // four warps share a row's parts when each gets two or more (37 parts of 512 rows x 128: 4.0 us against 12 us for a
+  // warp per row; two parts of 13312 rows x 128: 16 us for a warp per row against 30 us)
+  if (a.splits >= 8) {
+    cfg.gridDim = dim3((unsigned)a.part_rows);
+    NB_LAUNCH("prefix_join", s, (void)cudaLaunchKernelEx(&cfg, prefix_join<T, 4>, a, lanes));
+  } else {
+    cfg.gridDim = dim3((unsigned)((a.part_rows + 3) / 4));
+    NB_LAUNCH("prefix_join", s, (void)cudaLaunchKernelEx(&cfg, prefix_join<T, 1>, a, lanes));
+  }
   return check_launch("prefix attention, joining the parts");
 }
 
@@ -321,7 +371,7 @@ int join(const PrefixArgs& a, cudaStream_t s) {
 int prefix_simt_splits(const PrefixArgs& a) {
   const int bm = simt_bm(a), bn = simt_bn(a);
   const long long blocks = ((a.tokens * a.G + bm - 1) / bm) * a.Hkv;
-  const long long want = blocks >= kSMs * 2 ? 1 : kSMs * 2 / blocks, most = (a.prefix + 4 * bn - 1) / (4 * bn);
+  const long long want = blocks >= kSMs * 2 ? 1 : std::min<long long>(kSMs * 2 / blocks, kMostParts), most = (a.prefix + 4 * bn - 1) / (4 * bn);
   const long long n = want < most ? want : most;
   return n < 1 ? 1 : (int)n;
 }
@@ -369,12 +419,14 @@ int choose(const natten_b200_prefix_geom* g, PrefixArgs* a, bool* tc) {
   *tc = g->path != NATTEN_B200_PATH_SIMT && why == nullptr;
   if (g->path == NATTEN_B200_PATH_TCGEN05 && !*tc)
     return set_error(NATTEN_B200_EINVAL, "prefix: shape not supported by the tcgen05 kernels: %s", why);
-  a->splits = *tc ? prefix_sm100_splits(*a) : prefix_simt_splits(*a);
+  if (*tc) prefix_sm100_plan(a);
+  else a->splits = prefix_simt_splits(*a);
+  a->part_rows = a->splits <= 1 ? 0 : a->cut > 0 ? a->cut * 256 : a->tokens * a->Hq;
   return NATTEN_B200_OK;
 }
 
 size_t scratch_bytes_of(const PrefixArgs& a) {
-  return a.splits <= 1 ? 0 : (size_t)a.splits * (size_t)a.tokens * a.Hq * ((size_t)a.D + 1) * sizeof(float);
+  return a.splits <= 1 ? 0 : (size_t)a.splits * (size_t)a.part_rows * ((size_t)a.D + 1) * sizeof(float);
 }
 
 }  // namespace
@@ -401,7 +453,8 @@ int natten_b200_prefix_forward(const natten_b200_prefix_geom* g, const void* q, 
     return set_error(NATTEN_B200_EINVAL, "prefix: null tensor");
   if ((window_out == nullptr) != (window_lse == nullptr))
     return set_error(NATTEN_B200_EINVAL, "prefix: window_out and window_lse must both be given or both be null");
-  for (const void* p : {q, k, v, (const void*)window_out, (const void*)out, (const void*)scratch})
+  if (((uintptr_t)scratch & 31) != 0) return set_error(NATTEN_B200_EINVAL, "prefix: scratch must be 32-byte aligned");
+  for (const void* p : {q, k, v, (const void*)window_out, (const void*)out})
     if (((uintptr_t)p & 15) != 0) return set_error(NATTEN_B200_EINVAL, "prefix: tensor pointers must be 16-byte aligned");
   bool tc;
   if (int rc = choose(g, &a, &tc)) return rc;
@@ -410,7 +463,7 @@ int natten_b200_prefix_forward(const natten_b200_prefix_geom* g, const void* q, 
     return set_error(NATTEN_B200_ERESOURCE, "prefix: scratch has %zu bytes, needs %zu", scratch == nullptr ? (size_t)0 : scratch_bytes, need);
   a.q = q; a.k = k; a.v = v; a.window_out = window_out; a.window_lse = window_lse; a.out = out; a.lse = lse;
   a.part_out = static_cast<float*>(scratch);
-  a.part_lse = a.part_out == nullptr ? nullptr : a.part_out + (size_t)a.splits * a.tokens * a.Hq * a.D;
+  a.part_lse = a.part_out == nullptr ? nullptr : a.part_out + (size_t)a.splits * a.part_rows * a.D;
   cudaStream_t s = (cudaStream_t)stream;
   set_last_path(tc ? "tcgen05" : "simt");
   if (int rc = tc ? run_prefix_sm100(a, g->dtype, s) : run_prefix_simt(a, g->dtype, s)) return rc;

@@ -4,10 +4,11 @@
 // so the prefix is read once for the batch.  A block owns two tiles of up to 128 rows and a range of 128-key chunks:
 //   TMA warp       Q tiles once, then K and V chunks into a ring of shared-memory slots (zero fill past the ends)
 //   MMA warp       S = Q K^T into tensor memory, O += P V with P from tensor memory (over S) and V MN-major
-//   8 softmax warps   one thread per row (four warps per tile): the chunk's maximum, P = 2^(scale S - m) rounded to the
-//                  tensors' type, the row's sum in float32; O stays in tensor memory for the whole range
-// While one tile's softmax runs the tensor core works for the other tile.  The reference maximum m of a row follows the
-// true one lazily: O and the sum are rescaled only when a chunk exceeds m by 2^8, so that P stays finite in either type.
+//   16 softmax warps   eight per tile, two threads per row, each with half of the chunk's keys: the row's maximum, P =
+//                  2^(scale S - m) rounded to the tensors' type, the sum in float32; O stays in tensor memory throughout
+// While one tile's softmax runs the tensor core works for the other tile.  A block that has one tile only lets its two
+// halves take every other chunk for it.  The reference maximum m of a row follows the true one lazily: O and the sum are
+// rescaled only when a chunk exceeds m by 2^8, so that P stays finite in either type.
 #include <cuda.h>
 #include <math.h>
 
@@ -24,13 +25,17 @@ using namespace sm100;
 
 constexpr int kSMs = 148;
 constexpr int kRows = 128;               // rows of a tile = lanes of tensor memory
-constexpr int kKeys = 128;               // keys of a chunk
-constexpr int kThreads = 320;
-constexpr int kBlk = kRows * 128;        // bytes of 128 rows x 64 channels, one 128-byte swizzled row each
-constexpr int kMaxSlots = 8;
+constexpr int kSteps = 8;               // barriers of the ring, by step
+// For heads padded to DP channels: keys of a chunk, threads per row and keys of each, buffers of S / P for a tile, and the
+// threads of a block (the softmax warps of two tiles, a warp that loads, a warp that issues the products).
+template <int DP> struct Shape {
+  static constexpr int kKeys = DP == 64 ? 96 : 128, kBufs = DP == 64 ? 2 : 1, kSplit = DP == 64 ? 2 : 1, kEach = kKeys / kSplit;
+  static constexpr int kSoftmax = 256 * kSplit, kThreads = kSoftmax + 64;
+  static constexpr uint32_t kOCol = 2 * kBufs * kKeys;       // tensor memory: S / P of the tiles, then their O
+  static_assert(kOCol + 2 * DP <= 512, "tensor memory");
+};
 constexpr float kLazy = 8.f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr uint32_t kOCol = 256;          // tensor memory: S / P of tile t at column t * 128, O at 256 + t * 128
 
 struct alignas(64) PrefixMaps {
   CUtensorMap q, k, v;
@@ -41,20 +46,56 @@ struct PrefixTc {
   int tile_tokens;                       // query tokens of a tile: 128 / G
   long long tiles;                       // row tiles of a key/value head
   int pairs;                             // blocks of two tiles
+  int whole, cut;                        // work items that are one block's, and items that are cut into parts
+  int q_tiles;                           // Q tiles in shared memory: 1 when no block has two
   int slots;                             // ring slots of one K or V chunk
   int chunks;
   float scale_log2;
   int* status;
 };
 
-enum { B_Q = 0, B_FULL = 1, B_EMPTY = B_FULL + kMaxSlots, B_S = B_EMPTY + kMaxSlots, B_P = B_S + 2, B_PV = B_P + 2, B_DRAIN = B_PV + 2, B_COUNT };
+struct Results {
+  float sums[2][2][kRows], refs[2][kRows];                  // by stream and part of the keys; by stream
+};
+
+enum { B_Q = 0, B_FULL = 1, B_EMPTY = B_FULL + kSteps, B_S = B_EMPTY + kSteps, B_P = B_S + 4, B_PV = B_P + 4, B_COUNT = B_PV + 4 };
+
+template <int kBufs> struct Shared {
+  float peak[kBufs][2][2][kRows];                           // a chunk's maximum by buffer, stream, half of the keys and row
+  uint64_t bars[B_COUNT];
+  uint32_t tmem_slot;
+  int abort_word, limit_word;
+};
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-
+// Largest of three; NaN if one of them is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// Pairs of floats: one instruction for both.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair(float lo, float hi) {
+  f32x2 d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+__device__ __forceinline__ void unpair(f32x2 v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
   if constexpr (BF16) {
@@ -81,6 +122,30 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
         "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr)
       : "memory");
+}
+
+__device__ __forceinline__ void store32(float* p, const float* v) {
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]),
+               "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+               : "memory");
+}
+
+// For the many warps that wait for a product: each try suspends the warp for a short while, so that waiting takes few issue
+// slots from the warps that compute.
+__device__ __forceinline__ bool wait_softly(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+#pragma unroll 1
+  for (uint32_t it = 0; it < kPollLimit; ++it) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred P1;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 P1, [%1], %2, %3;\n\t"
+        "selp.b32 %0, 1, 0, P1;\n\t}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(20u)
+        : "memory");
+    if (ok) return true;
+  }
+  return mbar_wait(bar, parity, abort_flag);
 }
 
 // Sum over the keys [key0, key1) of one row, computed by a whole warp from global memory: for rows of a chunk in which
@@ -116,88 +181,127 @@ __device__ __noinline__ void row_alone(const PrefixArgs& a, long long token, int
 }
 
 template <int DP, bool BF16>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Shape<DP>::kThreads, 1)
 prefix_sm100(const __grid_constant__ PrefixTc p, const __grid_constant__ PrefixMaps maps) {
   constexpr int NB = DP / 64;                               // 64-channel blocks of a row
-  constexpr uint32_t kTileBytes = NB * kBlk;                // a Q tile, a K chunk, a V chunk
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  uint8_t* ring = smem + 2 * kTileBytes;
-  __shared__ uint64_t bars[B_COUNT];
-  __shared__ uint32_t tmem_slot;
-  __shared__ int abort_word, limit_word;
-  volatile int* abort_flag = &abort_word;
+  typedef Shape<DP> Sh;
+  constexpr int kKeys = Sh::kKeys, kSplit = Sh::kSplit, kEach = Sh::kEach, kBufs = Sh::kBufs, kWarps = Sh::kSoftmax / 32;
+  constexpr uint32_t kOCol = Sh::kOCol;
+  constexpr uint32_t kQBlk = kRows * 128, kBlk = kKeys * 128;      // bytes of 64 channels of a Q tile and of a chunk
+  constexpr uint32_t kQBytes = NB * kQBlk, kTileBytes = NB * kBlk; // a Q tile; a K or V chunk
+  // The tiles come first: they need 1024-byte alignment, which the start of a block's shared memory has, and with a
+  // 128-channel ring of five slots there is no room to round it up.
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint8_t* ring = smem + p.q_tiles * kQBytes;
+  Shared<kBufs>& sh = *reinterpret_cast<Shared<kBufs>*>(ring + p.slots * kTileBytes);
+  Results& res = *reinterpret_cast<Results*>(smem);         // over Q, once every product is done
+  volatile int* abort_flag = &sh.abort_word;
 
   const PrefixArgs& a = p.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const uint32_t bar0 = smem_u32(bars);
+  const uint32_t bar0 = smem_u32(sh.bars);
   auto bar = [&](int i) { return bar0 + 8u * (uint32_t)i; };
 
-  // work item: row tiles run fastest, so that blocks that run together read the same keys
-  uint32_t w = blockIdx.x;
-  const int pair = (int)(w % (uint32_t)p.pairs); w /= (uint32_t)p.pairs;
-  const int split = (int)(w % (uint32_t)a.splits); w /= (uint32_t)a.splits;
-  const int hk = (int)w;
-  const int c0 = (int)((long long)p.chunks * split / a.splits);
-  int c1 = (int)((long long)p.chunks * (split + 1) / a.splits);
-  const int nt = (long long)pair * 2 + 1 < p.tiles ? 2 : 1;
+  // Work items are (row tile pair, key/value head), pairs running fastest so that blocks that run together read the
+  // same keys.  The first p.whole of them are a block's each, the others are cut into a.splits ranges of chunks.
+  const bool whole = blockIdx.x < (uint32_t)p.whole;
+  const uint32_t x = whole ? blockIdx.x : blockIdx.x - p.whole;
+  const int split = whole ? 0 : (int)(x % (uint32_t)a.splits), parts = whole ? 1 : a.splits;
+  const uint32_t item = whole ? x : p.whole + x / (uint32_t)a.splits;
+  const int hk = (int)(item / (uint32_t)p.pairs), pair_id = (int)(item - (uint32_t)hk * p.pairs);
+  const int c0 = (int)((long long)p.chunks * split / parts);
+  int c1 = (int)((long long)p.chunks * (split + 1) / parts);
+  // two streams of products: two tiles, each over all chunks, or (twin) one tile of which either stream takes every
+  // other chunk
+  const bool twin = (long long)pair_id * 2 + 1 >= p.tiles;
 
-  if (tid == 0) {
-    mbar_init(bar(B_Q), 1);
-    for (int i = 0; i < kMaxSlots; ++i) { mbar_init(bar(B_FULL + i), 1); mbar_init(bar(B_EMPTY + i), 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(bar(B_S + i), 1); mbar_init(bar(B_P + i), 4); mbar_init(bar(B_PV + i), 1); }
-    mbar_init(bar(B_DRAIN), 1);
-    abort_word = 0;
-    limit_word = 0;
-    mbar_fence_init();
-  }
-  __syncthreads();
-  if (warp == 9) {
-    tmem_alloc(smem_u32(&tmem_slot), 512);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the joining kernel may be set up meanwhile
+  // The loading warp sets the barriers up and goes on to load at once; the others meet when tensor memory is there.
+  if (warp == kWarps) {
+    if (lane == 0) {
+      mbar_init(bar(B_Q), 1);
+      for (int i = 0; i < kSteps; ++i) { mbar_init(bar(B_FULL + i), 1); mbar_init(bar(B_EMPTY + i), 1); }
+      for (int i = 0; i < 4; ++i) { mbar_init(bar(B_S + i), 1); mbar_init(bar(B_P + i), 4 * kSplit); mbar_init(bar(B_PV + i), 1); }
+      sh.abort_word = (smem_u32(smem) & 1023u) != 0 ? 1 : 0;  // every wait then gives up, and the status says so
+      sh.limit_word = 0;
+      mbar_fence_init();
+      tma_prefetch_desc(&maps.q);
+      tma_prefetch_desc(&maps.k);
+      tma_prefetch_desc(&maps.v);
+    }
+    __syncwarp();
+  } else if (warp == kWarps + 1) {
+    tmem_alloc(smem_u32(&sh.tmem_slot), 512);
     tmem_relinquish();
   }
-  // this thread's row (softmax warps)
-  const int tile = warp >> 2;                               // 0 or 1; 2 for the other warps
-  const int r = tid & 127;
+  // softmax threads: stream, half of the chunk's keys, row
+  const int stream = (warp / (4 * kSplit)) & 1, keys = kSplit == 1 ? 0 : (warp >> 2) & 1, r = tid & 127;
   long long token = 0;
   int head = 0, limit = 0;
   bool alive = false;
-  if (warp < 8) {
+  if (warp < kWarps) {
     const int tl = r / a.G;
-    token = ((long long)pair * 2 + tile) * p.tile_tokens + tl;
+    token = ((long long)pair_id * 2 + (twin ? 0 : stream)) * p.tile_tokens + tl;
     alive = tl < p.tile_tokens && token < a.tokens;
     head = hk * a.G + (r - tl * a.G);
     limit = alive ? prefix_limit(a, token) : 0;
-    if (a.lens != nullptr) {
-      const int most = __reduce_max_sync(0xffffffffu, limit);
-      if (lane == 0) atomicMax(&limit_word, most);
-    }
   }
   tc_fence_before();
-  __syncthreads();
+  if (a.lens != nullptr) {                                  // keys that no row of the block sees are left out
+    __syncthreads();
+    const int most = __reduce_max_sync(0xffffffffu, limit);
+    if (warp < kWarps && lane == 0) atomicMax(&sh.limit_word, most);
+    __syncthreads();
+    c1 = min(c1, (sh.limit_word + kKeys - 1) / kKeys);
+  } else if (warp == kWarps) {
+    __threadfence_block();
+    asm volatile("bar.arrive 10, %0;" ::"n"(Sh::kThreads) : "memory");
+  } else {
+    asm volatile("bar.sync 10, %0;" ::"n"(Sh::kThreads) : "memory");
+  }
   tc_fence_after();
-  const uint32_t tmem = tmem_slot;
-  if (a.lens != nullptr) c1 = min(c1, (limit_word + kKeys - 1) / kKeys);      // keys that no row of the block sees
+  const uint32_t tmem = warp == kWarps ? 0u : sh.tmem_slot;
   const int n = max(c1 - c0, 0);
+  // A stream has kBufs buffers of S / P, so Q K^T of its next chunks can run before P V of the present one.  Step s
+  // issues P V of chunk s and then Q K^T of chunk s + ahead, into the buffer that has become free; the steps before 0 are
+  // Q K^T alone.  V(s) and K(s + ahead) share a pair of barriers: full for both, and empty when Q K^T of chunk s + ahead is
+  // done, which runs last.
+  const int ahead = twin ? 2 * kBufs : kBufs;
 
-  if (warp == 8) {
+  if (warp == kWarps) {
     // ------------------------------------------------------------------ TMA producer
-    if (lane == 0 && n > 0) {
+    if (n > 0 && elect_one()) {
       bool ok = true;
-      mbar_arrive_expect_tx(bar(B_Q), (uint32_t)(nt * NB * 128 * a.G * p.tile_tokens));
-      for (int t = 0; t < nt; ++t)
+      mbar_arrive_expect_tx(bar(B_Q), (uint32_t)((twin ? 1 : 2) * NB * 128 * a.G * p.tile_tokens));
+      for (int t = 0; t < (twin ? 1 : 2); ++t)
         for (int b = 0; b < NB; ++b)
-          tma_load_3d(smem_u32(smem + t * kTileBytes + b * kBlk), &maps.q, bar(B_Q), b * 64, hk * a.G,
-                      (int)(((long long)pair * 2 + t) * p.tile_tokens));
-      uint32_t st = 0, par = 1u;
-      for (int i = 0; i < 2 * n; ++i) {                     // K and V of a chunk in turn
-        ok = mbar_wait(bar(B_EMPTY + st), par, abort_flag);
+          tma_load_3d(smem_u32(smem + t * kQBytes + b * kQBlk), &maps.q, bar(B_Q), b * 64, hk * a.G,
+                      (int)(((long long)pair_id * 2 + t) * p.tile_tokens));
+      // The q-th chunk to be loaded goes to slot q % slots.  It is free when the chunk q - slots has been used: in the
+      // step that chunk belongs to.
+      int q = 0, slot = 0, freed = -ahead;                  // steps before `freed` are known to be over
+      auto load = [&](const CUtensorMap* m, int c, int s) {
+        const int old = q - p.slots;
+        const int t = old < 0 ? -ahead - 1 : old < ahead ? old - ahead : (old - ahead) >> 1;
+        for (; ok && freed <= t; ++freed)
+          ok = mbar_wait(bar(B_EMPTY + ((freed + ahead) & (kSteps - 1))), (uint32_t)((freed + ahead) / kSteps) & 1u, abort_flag);
+        if (!ok) return;
+        for (int b = 0; b < NB; ++b)
+          tma_load_3d(smem_u32(ring + slot * kTileBytes + b * kBlk), m, bar(B_FULL + ((s + ahead) & (kSteps - 1))), b * 64, hk,
+                      (c0 + c) * kKeys);
+        ++q;
+        if (++slot == p.slots) slot = 0;
+      };
+      for (int s = -ahead; s < n && ok; ++s) {
+        const bool v = s >= 0, k = s + ahead < n;
+        // a barrier's phase of kSteps steps ago is over before its next one begins
+        for (; ok && freed <= s - kSteps; ++freed)
+          ok = mbar_wait(bar(B_EMPTY + ((freed + ahead) & (kSteps - 1))), (uint32_t)((freed + ahead) / kSteps) & 1u, abort_flag);
         if (!ok) break;
-        mbar_arrive_expect_tx(bar(B_FULL + st), kTileBytes);
-        const CUtensorMap* m = (i & 1) ? &maps.v : &maps.k;
-        for (int b = 0; b < NB; ++b)
-          tma_load_3d(smem_u32(ring + st * kTileBytes + b * kBlk), m, bar(B_FULL + st), b * 64, hk, (c0 + (i >> 1)) * kKeys);
-        if (++st == (uint32_t)p.slots) { st = 0; par ^= 1u; }
+        if (!v && !k) continue;
+        mbar_arrive_expect_tx(bar(B_FULL + ((s + ahead) & (kSteps - 1))), (v ? kTileBytes : 0u) + (k ? kTileBytes : 0u));
+        if (v) load(&maps.v, s, s);
+        if (ok && k) load(&maps.k, s + ahead, s);
       }
       if (!ok) {                                            // copies in flight land before the block gives its memory back
         const long long t0 = clock64();
@@ -205,192 +309,275 @@ prefix_sm100(const __grid_constant__ PrefixTc p, const __grid_constant__ PrefixM
       }
     }
     __syncwarp();
-  } else if (warp == 9) {
+  } else if (warp > kWarps) {
     // ------------------------------------------------------------------ MMA issuer
-    if (lane == 0 && n > 0) {
-      const uint32_t fmt = BF16 ? 1 : 0;
+    if (n > 0 && elect_one()) {
+      const int fmt = BF16 ? 1 : 0;
       const uint32_t idesc_qk = instr_desc(kRows, kKeys, fmt, 0, 0), idesc_pv = instr_desc(kRows, DP, fmt, 0, 1);
-      const uint64_t kdesc0 = smem_desc(0, 16, 1024, 2), vdesc0 = smem_desc(0, kBlk, 1024, 2);
-      const uint32_t q_lo = smem_u32(smem) >> 4, ring_lo = smem_u32(ring) >> 4;
-      uint32_t st = 0, par = 0;
-      auto next = [&]() { if (++st == (uint32_t)p.slots) { st = 0; par ^= 1u; } };
-      auto qk = [&](int t, uint32_t slot) {
-        const uint64_t ad = kdesc0 + q_lo + (uint32_t)t * (kTileBytes >> 4), bd = kdesc0 + ring_lo + slot * (kTileBytes >> 4);
+      const uint64_t kdesc0 = smem_desc(0, 16, 1024, 2) + (smem_u32(ring) >> 4), vdesc0 = smem_desc(0, kBlk, 1024, 2) + (smem_u32(ring) >> 4);
+      const uint64_t qdesc0 = smem_desc(0, 16, 1024, 2) + (smem_u32(smem) >> 4);
+      // One thread does all of this between two products, so its bookkeeping is kept to increments: a ready wait costs it
+      // about 90 cycles and every dependent instruction four or five, against 64 for a product.
+      constexpr uint32_t kTile16 = kTileBytes >> 4;
+      const uint32_t ring16 = (uint32_t)p.slots * kTile16;
+      uint32_t at = 0, full = 0, full_par = 0;
+      auto take = [&]() {
+        const uint32_t here = at;
+        at += kTile16;
+        if (at == ring16) at = 0;
+        return here;
+      };
+      auto loaded = [&]() {
+        const bool there = wait_softly(bar(B_FULL + full), full_par, abort_flag);
+        if (++full == kSteps) { full = 0; full_par ^= 1u; }
+        return there;
+      };
+      auto qk = [&](int e, int buf, uint32_t k_at) {
+        const uint64_t ad = qdesc0 + (twin ? 0u : (uint32_t)e * (kQBytes >> 4)), bd = kdesc0 + k_at;
+        const uint32_t to = tmem + (e * kBufs + buf) * kKeys;
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks)
-            mma_ss(tmem + t * 128, ad + b * (kBlk >> 4) + 2 * ks, bd + b * (kBlk >> 4) + 2 * ks, idesc_qk, b + ks > 0 ? 1u : 0u);
-        mma_commit(bar(B_S + t));
+            mma_ss(to, ad + b * (kQBlk >> 4) + 2 * ks, bd + b * (kBlk >> 4) + 2 * ks, idesc_qk, b + ks > 0 ? 1u : 0u);
+        mma_commit(bar(B_S + e * kBufs + buf));
       };
-      bool ok = mbar_wait(bar(B_Q), 0, abort_flag) && mbar_wait(bar(B_FULL + st), par, abort_flag);
-      if (ok) {
-        tc_fence_after();
-        for (int t = 0; t < nt; ++t) qk(t, st);
-        mma_commit(bar(B_EMPTY + st));
-        next();
-      }
-      for (int j = 0; j < n && ok; ++j) {
-        const uint32_t v_st = st, v_par = par;
-        next();
-        const uint32_t k_st = st, k_par = par;
-        const bool more = j + 1 < n;
-        if (more) next();
-        for (int t = 0; t < nt && ok; ++t) {
-          if (t == 0) ok = mbar_wait(bar(B_FULL + v_st), v_par, abort_flag);
-          ok = ok && mbar_wait_hot(bar(B_P + t), (uint32_t)j & 1u, abort_flag);
-          if (!ok) break;
-          tc_fence_after();
-          uint64_t bd = vdesc0 + ring_lo + v_st * (kTileBytes >> 4);
+      auto pv = [&](int e, int buf, uint32_t v_at, bool first) {
+        const uint32_t from = tmem + (e * kBufs + buf) * kKeys;
 #pragma unroll
-          for (int kk = 0; kk < kKeys / 16; ++kk)            // 16 keys: next 16 rows of V, next 8 columns of packed P
-            mma_ts(tmem + kOCol + t * 128, tmem + t * 128 + kk * 8, bd + kk * 128, idesc_pv, j + kk > 0 ? 1u : 0u);
-          mma_commit(bar(B_PV + t));
-          if (t == nt - 1) mma_commit(bar(B_EMPTY + v_st));
-          if (more) {
-            if (t == 0) ok = mbar_wait(bar(B_FULL + k_st), k_par, abort_flag);
-            if (!ok) break;
-            tc_fence_after();
-            qk(t, k_st);                                     // executes after P V, which has read P from the same columns
-            if (t == nt - 1) mma_commit(bar(B_EMPTY + k_st));
-          }
+        for (int kk = 0; kk < kKeys / 16; ++kk)              // 16 keys: next 16 rows of V, next 8 columns of packed P
+          mma_ts(tmem + kOCol + e * DP, from + (kk / (kEach / 16)) * kEach + (kk % (kEach / 16)) * 8, vdesc0 + v_at + kk * 128,
+                 idesc_pv, first && kk == 0 ? 0u : 1u);
+      };
+      bool ok = wait_softly(bar(B_Q), 0, abort_flag);
+      for (int c = 0; c < min(ahead, n) && ok; ++c) {
+        ok = loaded();
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t k_at = take();
+        if (twin) {
+          qk(c & 1, (c >> 1) & (kBufs - 1), k_at);
+        } else {
+          qk(0, c & (kBufs - 1), k_at);
+          qk(1, c & (kBufs - 1), k_at);
         }
       }
-      // every MMA is finished before tensor memory is given back
-      mma_commit(bar(B_DRAIN));
-      for (uint32_t i = 0; i < kSpinLimit; ++i)
-        if (mbar_try_wait(bar(B_DRAIN), 0)) break;
+      full = ahead;                                          // the step of chunk 0, also where there were fewer chunks
+      uint32_t buf = 0, p_par = 0;
+      for (int s = 0; s < n && ok; ++s) {
+        ok = loaded();
+        if (!ok) break;
+        const bool more = s + ahead < n;
+        const uint32_t v_at = take(), k_at = more ? take() : 0u;
+        const int e0 = twin ? s & 1 : 0, e1 = twin ? s & 1 : 1;        // the chunk's stream, or both
+#pragma unroll 1
+        for (int e = e0; e <= e1; ++e) {
+          ok = wait_softly(bar(B_P + e * kBufs + buf), p_par, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          pv(e, buf, v_at, twin ? s < 2 : s == 0);
+          if (more) qk(e, buf, k_at);                        // executes after P V, which has read P from the same columns
+          else mma_commit(bar(B_PV + e * kBufs + buf));      // no Q K^T follows to tell that this P V is done
+        }
+        if (!twin || (s & 1)) {                              // next chunk of the stream: other buffer, or next phase
+          if (kBufs == 1 || buf == 1) p_par ^= 1u;
+          buf = kBufs == 1 ? 0u : buf ^ 1u;
+        }
+      }
     }
     __syncwarp();
-  } else if (tile < nt) {
+  } else {
     // ------------------------------------------------------------------ softmax and epilogue
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_addr = tmem + lanes + tile * 128, o_addr = tmem + lanes + kOCol + tile * 128;
+    const uint32_t s_base = tmem + lanes + stream * kBufs * kKeys + keys * kEach, o_addr = tmem + lanes + kOCol + stream * DP;
+    const int mine = twin ? (n - stream + 1) / 2 : n;        // chunks of this stream
+    const int pair_bar = 1 + stream * 4 + (warp & 3);        // named barrier of the two warps that share 32 rows
     float m = -INFINITY, l = 0.f;
     bool ok = true;
-    for (int j = 0; j < n; ++j) {
-      ok = mbar_wait(bar(B_S + tile), (uint32_t)j & 1u, abort_flag);
-      if (!ok) break;
+    const bool tells = (twin || stream == 1) && keys == 0 && (warp & 3) == 0 && lane == 0;
+    int left = limit - (c0 + (twin ? stream : 0)) * kKeys - keys * kEach;       // keys of this half that the row sees
+    uint32_t buf = 0, par = 0;
+    for (int j = 0; j < mine; ++j, left -= twin ? 2 * kKeys : kKeys) {
+      ok = __all_sync(0xffffffffu, wait_softly(bar(B_S + stream * kBufs + buf), par, abort_flag));
+      // the chunk's keys have been used, and with them the step that held them
+      if (tells) mbar_arrive(bar(B_EMPTY + ((twin ? 2 * j + stream : j) & (kSteps - 1))));
+      if (!ok) {
+        // the warp beside may have passed and wait there
+        if (kSplit == 2) asm volatile("bar.arrive %0, 64;" ::"r"(pair_bar) : "memory");
+        break;
+      }
       tc_fence_after();
-      uint32_t s[128];
+      const uint32_t s_addr = s_base + buf * kKeys;
+      uint32_t s[kEach];
 #pragma unroll
-      for (int g = 0; g < 4; ++g) tmem_ld32(s_addr + g * 32, s + g * 32);
+      for (int g = 0; g < kEach / 32; ++g) tmem_ld32(s_addr + g * 32, s + g * 32);
+      if constexpr (kEach % 32 != 0) tmem_ld16(s_addr + kEach - 16, *reinterpret_cast<uint32_t(*)[16]>(s + kEach - 16));
       tmem_wait_ld();
-      const int left = limit - (c0 + j) * kKeys;             // keys of the chunk that the row sees
-      if (__any_sync(0xffffffffu, alive && left < kKeys)) {
+      if (__any_sync(0xffffffffu, alive && left < kEach)) {
 #pragma unroll
-        for (int i = 0; i < 128; ++i) s[i] = i < left ? s[i] : 0xff800000u;
+        for (int i = 0; i < kEach; ++i) s[i] = i < left ? s[i] : 0xff800000u;
       }
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int i = 0; i < 128; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(s[i]));
-      const float mc = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
-      const bool first = m == -INFINITY;
-      const bool bump = alive && !first && mc > m + kLazy;
+      for (int i = 0; i < kEach / 2; ++i) mx[i & 3] = max3(mx[i & 3], __uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
+      const float own = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
+      float mc = own * p.scale_log2;
+      if constexpr (kSplit == 2) {
+        // the other warp has read what stood here: it has handed over P since, or met this warp at the barrier once more
+        sh.peak[buf][stream][keys][r] = own;
+        asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
+        mc = max3(own, sh.peak[buf][stream][keys ^ 1][r], own) * p.scale_log2;
+      }
+      // a NaN counts as too far ahead, and ends in the row's result
+      const bool first = m == -INFINITY, bump = alive && !first && !(mc <= m + kLazy);
       if (__any_sync(0xffffffffu, bump)) {
-        // O is being accumulated by the P V of the chunk before: wait for it, then scale
-        ok = mbar_wait(bar(B_PV + tile), (uint32_t)(j - 1) & 1u, abort_flag);
-        if (!ok) break;
-        tc_fence_after();
+        // O has to be complete up to the chunk before.  With one buffer it is, as S of this chunk was issued after that
+        // P V; with two it is when S of the next chunk is there, or, at the end, when the P V says so itself.
+        if (kBufs == 2) {
+          const uint32_t other = stream * kBufs + (buf ^ 1u);          // of the chunk before and the next one
+          ok = j + 1 < mine ? mbar_wait(bar(B_S + other), buf == 1 ? par ^ 1u : par, abort_flag)
+                            : mbar_wait(bar(B_PV + other), 0, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
+          tc_fence_after();
+        }
         const float alpha = bump ? ex2(m - mc) : 1.f;
 #pragma unroll 1
-        for (int g = 0; g < DP / 16; ++g) {
+        for (int g = 0; ok && g < DP / 16 / kSplit; ++g) {       // each of the row's threads scales half of O
           uint32_t f[16];
-          tmem_ld16(o_addr + g * 16, f);
+          tmem_ld16(o_addr + keys * (DP / 2) + g * 16, f);
           tmem_wait_ld();
 #pragma unroll
           for (int i = 0; i < 16; ++i) f[i] = __float_as_uint(__uint_as_float(f[i]) * alpha);
-          tmem_st16(o_addr + g * 16, f);
+          tmem_st16(o_addr + keys * (DP / 2) + g * 16, f);
         }
-        tmem_wait_st();
         l *= alpha;
         if (bump) m = mc;
       }
       if (first) m = mc;
       const float base = m == -INFINITY ? 0.f : m;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      const f32x2 scale2 = pair(p.scale_log2, p.scale_log2), shift = pair(-base, -base);
+      f32x2 sum = pair(0.f, 0.f);
+      uint32_t pk[kEach / 2];
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        uint32_t pk[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float e0 = ex2(fmaf(__uint_as_float(s[g * 32 + 2 * i]), p.scale_log2, -base));
-          const float e1 = ex2(fmaf(__uint_as_float(s[g * 32 + 2 * i + 1]), p.scale_log2, -base));
-          sum[i & 3] += e0 + e1;
-          pk[i] = pack_pair<BF16>(e0, e1);
-        }
-        tmem_st16(s_addr + g * 16, pk);
+      for (int i = 0; i < kEach / 2; ++i) {
+        const f32x2 x = fma2(pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale2, shift);
+        float e0, e1;
+        unpair(x, e0, e1);
+        e0 = ex2(e0);
+        e1 = ex2(e1);
+        sum = add2(sum, pair(e0, e1));
+        pk[i] = pack_pair<BF16>(e0, e1);
+        if (i % 16 == 15) tmem_st16(s_addr + (i - 15), *reinterpret_cast<uint32_t(*)[16]>(pk + (i - 15)));
+        if (i % 16 == 7 && i + 1 == kEach / 2) tmem_st8(s_addr + (i - 7), *reinterpret_cast<uint32_t(*)[8]>(pk + (i - 7)));
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar(B_P + tile));
+      if (lane == 0) mbar_arrive(bar(B_P + stream * kBufs + buf));
+      if (kBufs == 1 || buf == 1) par ^= 1u;
+      buf = kBufs == 1 ? 0u : buf ^ 1u;
+      float s0, s1;
+      unpair(sum, s0, s1);
+      l += s0 + s1;
     }
-    if (ok && n > 0) ok = mbar_wait(bar(B_PV + tile), (uint32_t)(n - 1) & 1u, abort_flag);
+    if (!(m < INFINITY)) l = __int_as_float(0x7fffffff);     // a NaN or an infinity among the logits
+    // the last P V of both streams: nothing reads Q any more, and a twin's O is in two places
+    for (int e = 0; e < 2; ++e) {
+      const int of = twin ? (n - e + 1) / 2 : n;
+      if (of > 0) ok = mbar_wait(bar(B_PV + e * kBufs + (of - 1) % kBufs), 0, abort_flag) && ok;
+    }
+    ok = __all_sync(0xffffffffu, ok);
+    tc_fence_after();
+    res.sums[stream][keys][r] = l;
+    if (keys == 0) res.refs[stream][r] = m;
+    asm volatile("bar.sync 9, %0;" ::"n"(Sh::kSoftmax) : "memory");
+    // the row's result: of its stream, or of both streams joined
+    const int st0 = twin ? 0 : stream;
+    float f0 = 1.f, f1 = 0.f;
+    l = res.sums[st0][0][r] + (kSplit == 2 ? res.sums[st0][1][r] : 0.f);
+    m = res.refs[st0][r];
+    if (twin && n > 1) {
+      const float m1 = res.refs[1][r], l1 = res.sums[1][0][r] + (kSplit == 2 ? res.sums[1][1][r] : 0.f);
+      const float top = fmaxf(m, m1), base = top == -INFINITY ? 0.f : top;
+      f0 = ex2(m - base);
+      f1 = ex2(m1 - base);
+      l = (f0 != 0.f ? l * f0 : 0.f) + (f1 != 0.f ? l1 * f1 : 0.f);
+      m = top;
+    }
     if (ok) {
-      tc_fence_after();
-      const bool last = a.splits == 1;
+      typedef typename std::conditional<BF16, __nv_bfloat16, __half>::type T;
       const long long at = token * a.Hq + head;
+      // a part's row in the buffers that the parts are joined from
+      const long long prow = ((long long)split * p.cut + (item - p.whole)) * (2 * kRows) + (twin ? 0 : stream * kRows) + r;
       float lse = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
       float wa = 1.f, wb = 0.f;
-      const bool win = last && a.window_lse != nullptr;
+      const bool win = whole && a.window_lse != nullptr;
       if (win && alive) lse = join_weights(lse, a.window_lse[at], wa, wb);
       const float co = l == 0.f ? 0.f : wa / l;              // a NaN sum stays one
-      bool odd = false;
+      const float co0 = f0 != 0.f ? co * f0 : 0.f, co1 = f1 != 0.f ? co * f1 : 0.f;
+      const bool o_none = !(co0 != 0.f) || n == 0, both = twin && n > 1;      // O of a row without keys may hold anything
+      // this thread's columns of the row
+      const int width = DP / kSplit / (twin ? 2 : 1), first_col = (twin ? stream * kSplit + keys : keys) * width;
+      const uint32_t o0 = tmem + lanes + kOCol + st0 * DP;
+      float check = 0.f;                                     // becomes NaN with any value that is not finite
 #pragma unroll 1
-      for (int g = 0; g < DP / 16; ++g) {
-        uint32_t f[16];
-        if (n > 0) {
-          tmem_ld16(o_addr + g * 16, f);
-          tmem_wait_ld();
+      for (int col = first_col; col < first_col + width; col += 16) {
+        uint32_t f[16], f2[16];
+        tmem_ld16(o0 + col, f);
+        if (both) tmem_ld16(o0 + DP + col, f2);
+        tmem_wait_ld();
+        if (!alive || col >= a.D) continue;                  // head dims are multiples of 8
+        float v[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = o_none ? 0.f : __uint_as_float(f[i]) * co0;
+        if (both && co1 != 0.f) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] = fmaf(__uint_as_float(f2[i]), co1, v[i]);
+        }
+        const int cols = min(16, a.D - col);
+        if (a.lens != nullptr) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) check += i < cols ? v[i] - v[i] : 0.f;
         }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float v = co != 0.f && n > 0 ? __uint_as_float(f[i]) * co : 0.f;
-          odd = odd || (co != 0.f && !isfinite(v) && g * 16 + i < a.D);
-          f[i] = __float_as_uint(v);
-        }
-        if (alive) {
+        for (int h8 = 0; h8 < 2; ++h8) {
+          if (h8 * 8 >= cols) break;
+          const float* u = v + h8 * 8;
+          const int c = col + h8 * 8;
+          if (!whole) {
+            // a whole 32-byte sector at once
+            store32(a.part_out + prow * a.D + c, u);
+            continue;
+          }
+          float o[8];
 #pragma unroll
-          for (int h8 = 0; h8 < 2; ++h8) {
-            const int c = g * 16 + h8 * 8;
-            if (c >= a.D) break;                             // head dims are multiples of 8
-            if (last) {
-              if (win && wb != 0.f) {
-                const uint4 raw = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.window_out) + at * a.D + c));
-                const uint32_t rw[4] = {raw.x, raw.y, raw.z, raw.w};
+          for (int i = 0; i < 8; ++i) o[i] = u[i];
+          if (win && wb != 0.f) {
+            const uint4 raw = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.window_out) + at * a.D + c));
+            const uint32_t rw[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  const float2 o = unpack_pair<BF16>(rw[i]);
-                  f[h8 * 8 + 2 * i] = __float_as_uint(fmaf(wb, o.x, __uint_as_float(f[h8 * 8 + 2 * i])));
-                  f[h8 * 8 + 2 * i + 1] = __float_as_uint(fmaf(wb, o.y, __uint_as_float(f[h8 * 8 + 2 * i + 1])));
-                }
-              }
-              uint32_t pk[4];
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                pk[i] = pack_pair<BF16>(__uint_as_float(f[h8 * 8 + 2 * i]), __uint_as_float(f[h8 * 8 + 2 * i + 1]));
-              *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + at * a.D + c) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
-            } else {
-              float* dst = a.part_out + ((long long)split * a.tokens * a.Hq + at) * a.D + c;
-              *reinterpret_cast<uint4*>(dst) = make_uint4(f[h8 * 8], f[h8 * 8 + 1], f[h8 * 8 + 2], f[h8 * 8 + 3]);
-              *reinterpret_cast<uint4*>(dst + 4) = make_uint4(f[h8 * 8 + 4], f[h8 * 8 + 5], f[h8 * 8 + 6], f[h8 * 8 + 7]);
+            for (int i = 0; i < 4; ++i) {
+              const float2 ow = unpack_pair<BF16>(rw[i]);
+              o[2 * i] = fmaf(wb, ow.x, o[2 * i]);
+              o[2 * i + 1] = fmaf(wb, ow.y, o[2 * i + 1]);
             }
           }
+          uint32_t pk[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) pk[i] = pack_pair<BF16>(o[2 * i], o[2 * i + 1]);
+          *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + at * a.D + c) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
         }
       }
-      if (alive) {
-        if (!last) a.part_lse[(long long)split * a.tokens * a.Hq + at] = lse;
+      if (alive && first_col == 0) {
+        if (!whole) a.part_lse[prow] = lse;
         else if (a.lse != nullptr) a.lse[at] = lse;
       }
       // rows whose keys end inside the block's range and that met a non-finite value past their end
-      uint32_t again = __ballot_sync(0xffffffffu, a.lens != nullptr && alive && odd && limit < c1 * kKeys);
-      typedef typename std::conditional<BF16, __nv_bfloat16, __half>::type T;
+      uint32_t again = __ballot_sync(0xffffffffu, a.lens != nullptr && alive && check != 0.f && limit < c1 * kKeys);
       while (again != 0) {
         const int who = __ffs(again) - 1;
         again &= again - 1;
-        const long long tok = __shfl_sync(0xffffffffu, token, who);
+        const long long tok = __shfl_sync(0xffffffffu, token, who), pr = __shfl_sync(0xffffffffu, prow, who);
         const int h = __shfl_sync(0xffffffffu, head, who), lim = __shfl_sync(0xffffffffu, limit, who);
         const float mm = __shfl_sync(0xffffffffu, m, who), cc = __shfl_sync(0xffffffffu, co, who), bb = __shfl_sync(0xffffffffu, wb, who);
         float acc[4];
@@ -399,13 +586,13 @@ prefix_sm100(const __grid_constant__ PrefixTc p, const __grid_constant__ PrefixM
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int c = i * 32 + lane;
-          if (c < a.D) {
+          if (c >= first_col && c < first_col + width && c < a.D) {
             float v = acc[i] * cc;
-            if (last) {
+            if (whole) {
               if (win && bb != 0.f) v = fmaf(bb, to_f<T>(static_cast<const T*>(a.window_out)[row * a.D + c]), v);
               static_cast<T*>(a.out)[row * a.D + c] = from_f<T>(v);
             } else {
-              a.part_out[((long long)split * a.tokens * a.Hq + row) * a.D + c] = v;
+              a.part_out[pr * a.D + c] = v;
             }
           }
         }
@@ -415,7 +602,7 @@ prefix_sm100(const __grid_constant__ PrefixTc p, const __grid_constant__ PrefixM
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == kWarps + 1) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
@@ -441,16 +628,19 @@ int encode_rows(CUtensorMap* map, const void* base, int dtype, int D, int heads,
 
 template <int DP, bool BF16>
 int launch(const PrefixTc& p, const PrefixMaps& maps, cudaStream_t s) {
-  const size_t tile = (size_t)(DP / 64) * kBlk, smem = 1024 + 2 * tile + (size_t)p.slots * tile;
+  const size_t smem = (size_t)DP * 2 * (p.q_tiles * kRows + p.slots * Shape<DP>::kKeys) + sizeof(Shared<Shape<DP>::kBufs>);
   const cudaError_t e = cudaFuncSetAttribute(prefix_sm100<DP, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) {
     (void)cudaGetLastError();
     return set_error(NATTEN_B200_ELAUNCH, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
   }
-  const long long grid = (long long)p.pairs * p.a.splits * p.a.Hkv;
-  NB_LAUNCH("prefix_sm100", s, prefix_sm100<DP, BF16><<<(unsigned)grid, kThreads, smem, s>>>(p, maps));
+  const long long grid = p.whole + (long long)p.cut * p.a.splits;
+  NB_LAUNCH("prefix_sm100", s, prefix_sm100<DP, BF16><<<(unsigned)grid, Shape<DP>::kThreads, smem, s>>>(p, maps));
   return check_launch("prefix attention (tensor cores)");
 }
+
+int chunk_keys(const PrefixArgs& a) { return a.D <= 64 ? Shape<64>::kKeys : Shape<128>::kKeys; }
+int chunks_of(const PrefixArgs& a) { return (a.prefix + chunk_keys(a) - 1) / chunk_keys(a); }
 
 long long row_tiles(const PrefixArgs& a) {
   const int tt = kRows / a.G;
@@ -471,18 +661,25 @@ const char* prefix_sm100_unsupported(const PrefixArgs& a, int dtype) {
   return nullptr;
 }
 
-// Parts of the prefix.  A block takes about one unit of time per chunk of 128 keys and about three to start and finish;
-// the blocks run in waves of one per SM, and joining parts costs another launch.
-int prefix_sm100_splits(const PrefixArgs& a) {
-  const long long items = (row_tiles(a) + 1) / 2 * a.Hkv, chunks = (a.prefix + kKeys - 1) / kKeys;
-  long long best = 1;
-  double best_cost = 1e300;
-  for (long long n = 1; n <= chunks && n <= 256 && (n == 1 || items * n <= 2 * kSMs); ++n) {
-    const double waves = (double)((items * n + kSMs - 1) / kSMs);
-    const double cost = waves * ((double)((chunks + n - 1) / n) + 3.0) + (n > 1 ? 3.0 + 0.02 * (double)n : 0.0);
-    if (cost < best_cost) { best_cost = cost; best = n; }
+// How the work items are spread over the SMs.  They run in waves of one block per slot; of the items that do not fill the
+// last wave, or of all when there are few, each is cut into parts, whose results a second kernel joins.  In units of a
+// chunk's time a block costs its chunks and about four to start and finish, the joining about three.
+void prefix_sm100_plan(PrefixArgs* a) {
+  const long long slots = kSMs;
+  const long long items = (row_tiles(*a) + 1) / 2 * a->Hkv, chunks = chunks_of(*a), waves = items / slots;
+  double best = 1e300;
+  for (long long back = 0; back <= 1 && back <= waves; ++back) {
+    const long long whole = (waves - back) * slots, rest = items - whole;
+    for (long long n = 1; n <= chunks && n <= 256 && (n == 1 || rest * n <= 2 * slots); ++n) {
+      const double cost = (double)(waves - back) * (double)(chunks + 4) + (double)((rest * n + slots - 1) / slots) * (double)((chunks + n - 1) / n + 4) +
+                          (n > 1 && rest > 0 ? 3.0 : 0.0);
+      if (cost < best) {
+        best = cost;
+        a->splits = rest > 0 ? (int)n : 1;
+        a->cut = n > 1 ? rest : 0;
+      }
+    }
   }
-  return (int)best;
 }
 
 int run_prefix_sm100(const PrefixArgs& a, int dtype, cudaStream_t s) {
@@ -491,15 +688,18 @@ int run_prefix_sm100(const PrefixArgs& a, int dtype, cudaStream_t s) {
   p.tile_tokens = kRows / a.G;
   p.tiles = row_tiles(a);
   p.pairs = (int)((p.tiles + 1) / 2);
-  p.chunks = (a.prefix + kKeys - 1) / kKeys;
-  p.slots = a.D <= 64 ? 8 : 5;
+  p.chunks = chunks_of(a);
+  p.cut = (int)a.cut;
+  p.whole = p.pairs * a.Hkv - p.cut;
+  p.q_tiles = p.tiles > 1 ? 2 : 1;
+  p.slots = a.D <= 64 ? 14 : 7 - p.q_tiles;   // what fits beside Q
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.status = sm100_status_word();
   if (p.status == nullptr) return set_error(NATTEN_B200_ENODEVICE, "tensor-core kernels need an sm_100 device");
   PrefixMaps maps;
   if (int rc = encode_rows(&maps.q, a.q, dtype, a.D, a.Hq, a.tokens, a.q_head, a.q_token, a.G, p.tile_tokens)) return rc;
-  if (int rc = encode_rows(&maps.k, a.k, dtype, a.D, a.Hkv, a.prefix, a.k_head, a.k_token, 1, kKeys)) return rc;
-  if (int rc = encode_rows(&maps.v, a.v, dtype, a.D, a.Hkv, a.prefix, a.v_head, a.v_token, 1, kKeys)) return rc;
+  if (int rc = encode_rows(&maps.k, a.k, dtype, a.D, a.Hkv, a.prefix, a.k_head, a.k_token, 1, chunk_keys(a))) return rc;
+  if (int rc = encode_rows(&maps.v, a.v, dtype, a.D, a.Hkv, a.prefix, a.v_head, a.v_token, 1, chunk_keys(a))) return rc;
   const bool bf = dtype == NATTEN_B200_BF16;
   if (a.D <= 64) return bf ? launch<64, true>(p, maps, s) : launch<64, false>(p, maps, s);
   return bf ? launch<128, true>(p, maps, s) : launch<128, false>(p, maps, s);

@@ -4,8 +4,8 @@ result, splitting, strides, refusals.
 
 Tolerances.  Let u be half a step of the type, e = 2^-24, o = sum w v with weights w that sum to 1, A = sum w |v|.
 A logit is a sum of D products in float32: off by at most 2 (D + 2) e scale sum |q k| (the factor 2: the tensor core may
-truncate where it adds), which with 2^-21 for the base-2 exponential and its argument is the relative error r of a
-weight.  On the tensor cores a weight is also rounded to the type (u; fp16 steps no finer than 2^-24 below 2^-14, against a
+truncate where it adds), which with 2^-18 for the base-2 exponential (a polynomial of 2^-18.5 on the tensor
+cores' path) and its argument is the relative error r of a weight.  On the tensor cores a weight is also rounded to the type (u; fp16 steps no finer than 2^-24 below 2^-14, against a
 sum of at least 1: 2^-25 for each key, times |v|).  Sums over n keys are tree-like or at most 2 (n / 16 + 64) e.  So
   |out - o| <= u |o| + (2 r + u + 2 (n / 16 + 64) e) A + 2 e |o|,   |lse - l| <= r + 2 (n / 16 + 64) e + 4 e |l|."""
 
@@ -46,7 +46,7 @@ def _definition(q, k, v, scale, lens=None, window=None, tc=True):
             kh, vh = k[:m, h // (hq // hk)], v[:m, h // (hq // hk)]
             s = flat[i, :, h] @ kh.T * scale
             w = torch.softmax(s, -1)
-            r = 2 * (d + 2) * E * scale * (flat[i, :, h].abs() @ kh.abs().T).amax(-1) + 2.0 ** -21
+            r = 2 * (d + 2) * E * scale * (flat[i, :, h].abs() @ kh.abs().T).amax(-1) + 2.0 ** -18
             out[i, :, h], lse[i, :, h] = w @ vh, torch.logsumexp(s, -1)
             sums = 2 * (m / 16 + 64) * E
             o_err[i, :, h] = (2 * r + u + sums).unsqueeze(-1) * (w @ vh.abs()) + 2 * E * out[i, :, h].abs()
@@ -110,7 +110,8 @@ TC = [
     ((1, 1, 1, 64), 1, 1), ((1, 1, 1, 8), 1, 127), ((2, 1, 8, 64), 2, 128), ((3, 1, 4, 128), 4, 129), ((64, 1, 16, 64), 4, 300),
     ((1, 130, 2, 64), 2, 257), ((2, 9, 15, 4, 32), 4, 200), ((1, 5, 7, 11, 3, 24), 1, 385), ((2, 300, 6, 128), 2, 1000),
     ((1, 257, 1, 80), 1, 640), ((5, 3, 7, 128), 1, 131), ((2, 3, 130, 16), 2, 90), ((1, 2, 128, 40), 1, 77), ((1, 700, 5, 72), 5, 140),
-    ((1, 1, 2, 128), 1, 20000), ((4, 1, 8, 64), 8, 6000),
+    ((1, 1, 2, 128), 1, 20000), ((4, 1, 8, 64), 8, 6000), ((1, 2100, 18, 64), 18, 1500), ((1, 1300, 8, 104), 8, 800),
+    ((40, 33, 8, 32), 8, 2000),
 ]
 
 
@@ -124,7 +125,7 @@ def test_tensor_core_kernel(shape, hk, n, dtype):
 SIMT = [
     ((1, 1, 1, 1), 1, 1), ((2, 1, 8, 64), 2, 63), ((3, 1, 4, 128), 4, 65), ((2, 9, 15, 4, 32), 4, 200), ((1, 5, 7, 3, 24), 1, 385),
     ((1, 130, 2, 17), 2, 257), ((1, 70, 4, 200), 2, 99), ((1, 1, 2, 256), 1, 3001), ((1, 90, 1, 256), 1, 33), ((2, 40, 3, 130), 1, 64),
-    ((16, 1, 2, 66), 2, 500), ((1, 1, 300, 12), 2, 40),
+    ((16, 1, 2, 66), 2, 500), ((1, 1, 300, 12), 2, 40), ((1, 1, 1, 150), 1, 40000), ((1, 2, 2, 131), 2, 5000),
 ]
 
 
@@ -343,7 +344,7 @@ def test_abi_pointers_and_scratch():
     assert lib.natten_b200_prefix_forward(_geom(), 4096 + 8, 4096, 4096, None, None, 4096, None, None, 0, None) == _lib.EINVAL
     long = _geom(prefix=100000)
     need = lib.natten_b200_prefix_scratch_bytes(long)
-    assert need > 0 and need % (2 * 3 * 4 * 65 * 4) == 0
+    assert need > 0 and need % (65 * 4) == 0
     assert lib.natten_b200_prefix_forward(long, 4096, 4096, 4096, None, None, 4096, None, 4096, need - 1, None) == _lib.ERESOURCE
     assert lib.natten_b200_prefix_forward(long, 4096, 4096, 4096, None, None, 4096, None, None, 0, None) == _lib.ERESOURCE
     assert lib.natten_b200_prefix_forward(_geom(batch=0), None, None, None, None, None, None, None, None, 0, None) == _lib.OK
