@@ -4,7 +4,8 @@
 
 Each ``csrc/*.cu`` is compiled to an object (in parallel, skipped when the
 object is newer than every source and header) and linked into
-``natten_mlx_b200/libnatten_b200.so``.  No GPU is needed to build.
+``natten_mlx_b200/libnatten_b200.so``.  ``csrc/torch_binding.cpp`` becomes the extension module
+``natten_mlx_b200/_torch_binding.*.so``, against the headers of the torch that runs the build.  No GPU is needed to build.
 """
 
 from __future__ import annotations
@@ -14,11 +15,13 @@ import glob
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "build")
 OUT = os.path.join(HERE, "natten_mlx_b200", "libnatten_b200.so")
+BINDING = os.path.join(HERE, "natten_mlx_b200", "_torch_binding" + sysconfig.get_config_var("EXT_SUFFIX"))
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
          "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr"] + os.environ.get("NATTEN_B200_NVCC_FLAGS", "").split()
@@ -56,7 +59,36 @@ def build(force: bool = False, verbose: bool = False) -> str:
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    build_binding(force)
     return OUT
+
+
+def build_binding(force: bool = False) -> str:
+    """The torch side of the operators that have one; rebuilt when its source, the C header or torch changed."""
+    import torch
+    from torch.utils.cpp_extension import include_paths
+
+    src = os.path.join(CSRC, "torch_binding.cpp")
+    stamp = os.path.join(OBJ, "torch_binding.version")
+    version = torch.__version__ + "\n" + sys.version
+    newest = _newest([src] + glob.glob(os.path.join(HERE, "..", "include", "*.h")))
+    old = open(stamp).read() if os.path.exists(stamp) else ""
+    if not force and old == version and os.path.exists(BINDING) and os.path.getmtime(BINDING) > newest:
+        return BINDING
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    includes = include_paths() + [sysconfig.get_paths()["include"], os.path.join(os.path.dirname(NVCC), "..", "include")]
+    # the host compiler that nvcc takes, and so the system's C++ runtime, which torch shares: one that links its own
+    # copy in (a CXX of another toolchain may) breaks the first stream of a number
+    cmd = (["g++", "-shared", "-fPIC", "-O2", "-std=c++17", "-fvisibility=hidden",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+           + [a for p in includes for a in ("-isystem", p)] + [src, "-o", BINDING]
+           + [f"-L{lib}", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_cuda", "-ldl"])
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on {src}:\n{r.stdout}\n{r.stderr}")
+    with open(stamp, "w") as fh:
+        fh.write(version)
+    return BINDING
 
 
 if __name__ == "__main__":

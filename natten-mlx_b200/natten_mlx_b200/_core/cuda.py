@@ -310,178 +310,6 @@ def merge_backward(o0, l0, o1, l1, grad_out, grad_lse):
 
 
 # ---------------------------------------------------------------------------
-# around the attention: layer norm, rotary positions, attention to a shared prefix
-#
-# These take a few microseconds on the device in serving, so the host side is kept short: no context manager while the
-# tensor's device is the current one, the raw stream handle, one allocation where two would do.
-# ---------------------------------------------------------------------------
-
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_current_device = torch.cuda.current_device
-
-
-def _elsewhere(device) -> bool:
-    return device.index != _current_device()
-
-
-def _strides(shape, stride):
-    """The axes as few (size, stride) pairs, outermost first: axes of one step are joined, those of size 1 dropped."""
-    pairs = []
-    for n, st in zip(shape, stride):
-        if n == 1:
-            continue
-        if pairs and pairs[-1][1] == n * st:
-            pairs[-1] = (pairs[-1][0] * n, st)
-        else:
-            pairs.append((n, st))
-    return pairs
-
-
-def _norm_rows(x):
-    """(x, natten_b200_rows): x itself when its rows follow one or two strides, else a dense copy."""
-    c = x.shape[-1]
-    if not x.is_contiguous():
-        pairs = _strides(x.shape[:-1], x.stride()[:-1]) if x.stride(-1) == 1 or c == 1 else ()
-        if len(pairs) == 1:
-            return x, _lib.Rows(x.numel() // c, 1, pairs[0][1], 0, c, 0)
-        if len(pairs) == 2:
-            return x, _lib.Rows(x.numel() // c, pairs[1][0], pairs[0][1], pairs[1][1], c, 0)
-        x = x.contiguous()
-    return x, _lib.Rows(x.numel() // c, 1, c, 0, c, 0)
-
-
-def _dense_like(x):
-    return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
-
-
-def layer_norm_forward(x, weight, bias, eps, save=False):
-    """Returns (y, stats): the means and then the reciprocal deviations of the rows, float32 ``[2, rows]``, or None
-    without ``save``."""
-    device = x.device
-    if _elsewhere(device):
-        with torch.cuda.device(device):
-            return layer_norm_forward(x, weight, bias, eps, save)
-    y = _dense_like(x)
-    x, rows = _norm_rows(x)
-    n = rows.rows
-    stats = torch.empty((2, n), dtype=torch.float32, device=device) if save else None
-    if n:
-        like = weight if weight is not None else bias if bias is not None else x
-        mean = 0 if stats is None else stats.data_ptr()
-        rc = _lib.load().natten_b200_layer_norm_forward(
-            _DTYPES[x.dtype], _DTYPES[like.dtype], rows, x.data_ptr(), _ptr(weight), _ptr(bias), eps, y.data_ptr(),
-            mean, mean and mean + 4 * n, _raw_stream(device.index))
-        if rc:
-            _lib.check(rc)
-    return y, stats
-
-
-def layer_norm_backward(x, weight, bias, stats, grad, want_dx, want_dw, want_db):
-    """Returns (dx, dweight, dbias), None for those that are not wanted."""
-    device = x.device
-    if _elsewhere(device):
-        with torch.cuda.device(device):
-            return layer_norm_backward(x, weight, bias, stats, grad, want_dx, want_dw, want_db)
-    like = weight if weight is not None else bias if bias is not None else x
-    dx = _dense_like(x) if want_dx else None
-    dw = torch.empty_like(weight) if want_dw else None
-    db = torch.empty_like(bias) if want_db else None
-    x, rows = _norm_rows(x)
-    if not grad.is_contiguous():
-        grad = grad.contiguous()
-    lib = _lib.load()
-    n, nbytes, scratch = rows.rows, 0, None
-    if want_dw or want_db:
-        nbytes = lib.natten_b200_layer_norm_backward_scratch_bytes(n, rows.channels)
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    mean = stats.data_ptr()
-    rc = lib.natten_b200_layer_norm_backward(
-        _DTYPES[x.dtype], _DTYPES[like.dtype], rows, x.data_ptr(), _ptr(weight), mean, mean + 4 * n, grad.data_ptr(),
-        _ptr(dx), _ptr(dw), _ptr(db), _ptr(scratch), nbytes, _raw_stream(device.index))
-    if rc:
-        _lib.check(rc)
-    return dx, dw, db
-
-
-def _token_head_strides(t):
-    """(t, token stride, head stride) of ``[..., heads, D]``: t itself when one stride leads through its tokens."""
-    heads, d = t.shape[-2:]
-    if not t.is_contiguous():
-        pairs = _strides(t.shape[:-2], t.stride()[:-2]) if t.stride(-1) == 1 or d == 1 else None
-        if pairs is not None and len(pairs) < 2:
-            return t, pairs[0][1] if pairs else heads * d, t.stride(-2) if heads > 1 else d
-        t = t.contiguous()
-    return t, heads * d, d
-
-
-def rotary(q, k, spec, origin, offsets, positions, inverse=0):
-    """Turns q and k; ``spec`` = (axes, axis_dims as three int32, phases as uint64, interleaved), ``origin`` three int64."""
-    device = q.device
-    if _elsewhere(device):
-        with torch.cuda.device(device):
-            return rotary(q, k, spec, origin, offsets, positions, inverse)
-    yq, yk = _dense_like(q), _dense_like(k)
-    if not yq.numel():
-        return yq, yk
-    q, qt, qh = _token_head_strides(q)
-    k, kt, kh = _token_head_strides(k)
-    shape = q.shape
-    rank = len(shape) - 3
-    pos, kind = (positions, _lib.POS_GIVEN) if positions is not None else (offsets, _lib.POS_OFFSET)
-    if pos is None:
-        bits, batch, kind, where = 32, 0, _lib.POS_GRID, None
-    else:
-        bits, batch, where = 64 if pos.dtype == torch.int64 else 32, pos.shape[0] == shape[0], pos.data_ptr()
-    axes, axis_dims, phases, interleaved = spec
-    g = _lib.RotaryGeom(_DTYPES[q.dtype], rank, shape[0], (shape[1:-2] + (0, 0))[:3], shape[-2], k.shape[-2], shape[-1], axes,
-                        axis_dims, qt, qh, kt, kh, interleaved, kind, bits, batch, origin, where, ctypes.addressof(phases))
-    rc = _lib.load().natten_b200_rotary(g, q.data_ptr(), k.data_ptr(), yq.data_ptr(), yk.data_ptr(), inverse,
-                                        _raw_stream(device.index))
-    if rc:
-        _lib.check(rc)
-    return yq, yk
-
-
-def _tma_strides(t, d):
-    """As _token_head_strides, but a dense copy unless the strides and the address are multiples of 16 bytes."""
-    t, token, head = _token_head_strides(t)
-    step = 16 // t.element_size()
-    if t.data_ptr() % 16 or token < 1 or head < 1 or (not t.is_contiguous() and (token % step or head % step)):
-        t = t.clone(memory_format=torch.contiguous_format)
-        token, head = t.shape[-2] * d, d
-    return t, token, head
-
-
-def prefix_forward(q, k, v, scale, lens=None, window_out=None, window_lse=None, path=None):
-    """Returns (out, lse) of the queries over the shared prefix (and the window's keys)."""
-    device = q.device
-    if _elsewhere(device):
-        with torch.cuda.device(device):
-            return prefix_forward(q, k, v, scale, lens, window_out, window_lse, path)
-    d = q.shape[-1]
-    out = _dense_like(q)
-    lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=device)
-    if not out.numel():
-        return out, lse
-    q, qt, qh = _tma_strides(q, d)
-    k, kt, kh = _tma_strides(k, d)
-    v, vt, vh = _tma_strides(v, d)
-    if window_out is not None:
-        window_out, = _prep(window_out)
-    batch, heads = q.shape[0], q.shape[-2]
-    g = _lib.PrefixGeom(_DTYPES[q.dtype], heads, k.shape[-2], d, batch, q.numel() // (batch * heads * d), k.shape[0],
-                        qt, qh, kt, kh, vt, vh, _scale(scale, d), _PATHS[_fused_path if path is None else path], _ptr(lens))
-    lib = _lib.load()
-    nbytes = lib.natten_b200_prefix_scratch_bytes(g)
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-    rc = lib.natten_b200_prefix_forward(g, q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(window_out), _ptr(window_lse),
-                                        out.data_ptr(), lse.data_ptr(), _ptr(scratch), nbytes, _raw_stream(device.index))
-    if rc:
-        _lib.check(rc)
-    return out, lse
-
-
-# ---------------------------------------------------------------------------
 # the backend-module protocol (names and argument order of the reference)
 # ---------------------------------------------------------------------------
 

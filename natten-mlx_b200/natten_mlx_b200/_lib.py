@@ -150,6 +150,25 @@ def load() -> ctypes.CDLL:
     return lib
 
 
+_binding = None
+
+
+def binding():
+    """The torch binding of the operators that have one (layer norm, rotary positions, attention to a shared prefix):
+    an extension module over the symbols of the library, with their autograd nodes."""
+    global _binding
+    if _binding is None:
+        load()
+        try:
+            from . import _torch_binding
+        except ImportError as exc:
+            raise ImportError("the torch binding is missing or does not fit this torch: build it with "
+                              "`python natten-mlx_b200/build.py`") from exc
+        _torch_binding.init(LIB_PATH)
+        _binding = _torch_binding
+    return _binding
+
+
 def last_error() -> str:
     return load().natten_b200_last_error().decode()
 

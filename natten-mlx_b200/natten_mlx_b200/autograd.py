@@ -10,7 +10,6 @@ the backward recomputes nothing but the softmax weights.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from ._core import ops
 from ._core import cuda as _cuda
@@ -107,53 +106,6 @@ class _Merge(torch.autograd.Function):
             grad_out = torch.zeros_like(o0)
         do0, dl0, do1, dl1 = _cuda.merge_backward(o0, l0, o1, l1, grad_out, grad_lse)
         return do0, dl0.to(l0.dtype), do1, dl1.to(l1.dtype)
-
-
-def _once(backward):
-    """A backward that cannot be differentiated itself.  Only a pass that builds a graph (``create_graph=True``) pays for
-    the wrapper that says so when that graph is used."""
-    guarded = once_differentiable(backward)
-
-    def call(ctx, *grads):
-        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
-    return call
-
-
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        y, stats = _cuda.layer_norm_forward(x, weight, bias, eps, True)
-        ctx.save_for_backward(x, weight, bias, stats)
-        return y
-
-    @staticmethod
-    @_once
-    def backward(ctx, grad):
-        need = ctx.needs_input_grad
-        return (*_cuda.layer_norm_backward(*ctx.saved_tensors, grad, need[0], need[1], need[2]), None)
-
-
-class _Rotary(torch.autograd.Function):
-    """The gradient of a turn is the turn back, so only the positions are kept."""
-
-    @staticmethod
-    def forward(ctx, q, k, spec, origin, offsets, positions):
-        ctx.save_for_backward(offsets, positions)
-        ctx.params = (spec, origin)
-        return _cuda.rotary(q, k, spec, origin, offsets, positions)
-
-    @staticmethod
-    @_once
-    def backward(ctx, grad_q, grad_k):
-        return (*_cuda.rotary(grad_q, grad_k, *ctx.params, *ctx.saved_tensors, 1), None, None, None, None)
-
-
-def layer_norm_with_grad(x, weight, bias, eps):
-    return _LayerNorm.apply(x, weight, bias, eps)
-
-
-def rotary_with_grad(q, k, spec, origin, offsets, positions):
-    return _Rotary.apply(q, k, spec, origin, offsets, positions)
 
 
 def fused_with_grad(q, k, v, ks, st, dl, ca, scale, k_extra=None, v_extra=None, sizes=None, host_sizes=None):

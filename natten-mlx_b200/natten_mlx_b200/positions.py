@@ -8,7 +8,6 @@ relative bias of its allin1 ops (src/natten_mlx/extras/allin1/__init__.py:40-79)
 
 from __future__ import annotations
 
-import ctypes
 import math
 from decimal import Decimal, localcontext
 from functools import lru_cache
@@ -16,13 +15,10 @@ from typing import Optional, Sequence, Tuple, Union
 
 import torch
 
-from . import autograd as _ag
-from ._core import cuda as _cuda
+from . import _lib
 from .utils.params import normalize_tuple_param
 
 _TWO_PI = Decimal("6.28318530717958647692528676655900576839433879875021164194988918461563281257241799725606965068")
-_NO_ORIGIN = (ctypes.c_int64 * 3)()
-_LAYOUTS = {1: "[B, L, heads, dim]", 2: "[B, H, W, heads, dim]", 3: "[B, D, H, W, heads, dim]"}
 
 
 def split_axis_dims(head_dim: int, axes: int) -> Tuple[int, ...]:
@@ -31,7 +27,6 @@ def split_axis_dims(head_dim: int, axes: int) -> Tuple[int, ...]:
     return (head_dim - head_dim % 2 - part * (axes - 1),) + (part,) * (axes - 1)
 
 
-@lru_cache(maxsize=128)
 def _phases(axis_dims: Tuple[int, ...], base: float, frequencies: Optional[Tuple[float, ...]]):
     """Angles per position as 64-bit fractions of a turn, computed with 50 digits."""
     with localcontext() as ctx:
@@ -40,25 +35,23 @@ def _phases(axis_dims: Tuple[int, ...], base: float, frequencies: Optional[Tuple
             rad = [Decimal(f) for f in frequencies]
         else:
             rad = [Decimal(base) ** (Decimal(-2 * j) / Decimal(d)) for d in axis_dims for j in range(d // 2)]
-        values = [int((f / _TWO_PI * (1 << 64)).to_integral_value()) % (1 << 64) for f in rad]
-    return (ctypes.c_uint64 * len(values))(*values)
+        return [int((f / _TWO_PI * (1 << 64)).to_integral_value()) % (1 << 64) for f in rad]
 
 
-@lru_cache(maxsize=128)
-def _spec(axis_dims: Tuple[int, ...], base: float, frequencies: Optional[Tuple[float, ...]], interleaved: bool):
-    """What a call hands to the library, once for each choice of arguments."""
-    dims = (ctypes.c_int32 * 3)(*axis_dims, *(0,) * (3 - len(axis_dims)))
-    return len(axis_dims), dims, _phases(axis_dims, base, frequencies), int(interleaved)
-
-
-def _check_positions(name, t, shape_ok, expected, query):
-    if not torch.is_tensor(t) or t.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"{name} must be an int32 or int64 tensor, got {t.dtype if torch.is_tensor(t) else type(t)}")
-    if not shape_ok:
-        raise ValueError(f"{name} must have shape {expected}, got {tuple(t.shape)}")
-    if t.device != query.device:
-        raise ValueError(f"{name} must be on the query's device {query.device}, got {t.device}")
-    return t.contiguous()
+@lru_cache(maxsize=256)
+def _spec(head_dim: int, axes: int, axis_dims: Optional[Tuple[int, ...]], base: float,
+          frequencies: Optional[Tuple[float, ...]], interleaved: bool):
+    """What a call hands to the library, checked and computed once for each choice of arguments."""
+    dims = split_axis_dims(head_dim, axes) if axis_dims is None else axis_dims
+    if not 1 <= len(dims) <= 3:
+        raise ValueError(f"axis_dims must have 1 to 3 entries, got {dims}")
+    if any(not isinstance(d, int) or d < 0 or d % 2 for d in dims) or not 2 <= sum(dims) <= min(head_dim, 512):
+        raise ValueError(f"axis_dims must be even, not negative and sum to 2..{min(head_dim, 512)}, got {dims}")
+    if not (base > 0.0 and math.isfinite(base)):
+        raise ValueError(f"base must be positive and finite, got {base}")
+    if frequencies is not None and (len(frequencies) != sum(dims) // 2 or not all(math.isfinite(f) for f in frequencies)):
+        raise ValueError(f"frequencies must be {sum(dims) // 2} finite numbers, got {len(frequencies)}")
+    return _lib.binding().RotarySpec(list(dims), _phases(dims, base, frequencies), interleaved)
 
 
 def rotary(query: torch.Tensor, key: torch.Tensor, axis_dims: Optional[Sequence[int]] = None, *, base: float = 10000.0,
@@ -82,55 +75,23 @@ def rotary(query: torch.Tensor, key: torch.Tensor, axis_dims: Optional[Sequence[
     (once) in query and key.
     """
     rank = query.dim() - 3
-    if rank not in (1, 2, 3) or key.dim() != query.dim():
-        raise ValueError("rotary expects query and key with one of the shapes " + ", ".join(_LAYOUTS.values()))
-    if query.shape[:-2] != key.shape[:-2]:
-        raise ValueError(f"Batch and spatial dimensions must match: Q={tuple(query.shape[:-2])}, K={tuple(key.shape[:-2])}.")
-    head_dim = query.shape[-1]
-    if key.shape[-1] != head_dim:
-        raise ValueError(f"Head dim must match: Q has {head_dim}, K has {key.shape[-1]}.")
-    if query.dtype not in _cuda._DTYPES or key.dtype != query.dtype:
-        raise ValueError(f"query and key must share a dtype of float32, float16 or bfloat16, got {query.dtype} and {key.dtype}")
-    if not query.is_cuda:
-        raise RuntimeError("natten_mlx_b200 runs on CUDA tensors only (there is no CPU path)")
-    if key.device != query.device:
-        raise ValueError("query and key must be on one device")
-    axes = rank if positions is None or axis_dims is not None else positions.shape[-1]
-    dims = split_axis_dims(head_dim, axes) if axis_dims is None else tuple(int(d) for d in axis_dims)
-    if not 1 <= len(dims) <= 3:
-        raise ValueError(f"axis_dims must have 1 to 3 entries, got {dims}")
-    if any(d < 0 or d % 2 for d in dims) or not 2 <= sum(dims) <= min(head_dim, 512):
-        raise ValueError(f"axis_dims must be even, not negative and sum to 2..{min(head_dim, 512)}, got {dims}")
-    base = float(base)
-    if not (base > 0.0 and math.isfinite(base)):
-        raise ValueError(f"base must be positive and finite, got {base}")
-    if frequencies is not None:
-        frequencies = tuple(float(f) for f in frequencies)
-        if len(frequencies) != sum(dims) // 2 or not all(math.isfinite(f) for f in frequencies):
-            raise ValueError(f"frequencies must be {sum(dims) // 2} finite numbers, got {len(frequencies)}")
-    origin, start = _NO_ORIGIN, None
+    if not 1 <= rank <= 3:
+        raise ValueError("rotary expects query and key with one of the shapes [B, L, heads, dim], [B, H, W, heads, dim], "
+                         "[B, D, H, W, heads, dim]")
+    origin, start = (), None
     if positions is not None:
         if offsets is not None:
             raise ValueError("offsets and positions cannot be combined")
-        lead = tuple(query.shape[1:-2])
-        ok = torch.is_tensor(positions) and positions.dim() == rank + 2 and positions.shape[0] in (1, query.shape[0]) \
-            and tuple(positions.shape[1:-1]) == lead and positions.shape[-1] == len(dims)
-        positions = _check_positions("positions", positions, ok, f"[{query.shape[0]} or 1, {lead}, {len(dims)}]", query)
-    else:
-        if len(dims) != rank:
-            raise ValueError(f"axis_dims must have an entry for each of the {rank} spatial axes, got {dims}")
-        if torch.is_tensor(offsets):
-            start = _check_positions("offsets", offsets, tuple(offsets.shape) == (query.shape[0], rank),
-                                     f"[{query.shape[0]}, {rank}]", query)
-        elif offsets is not None:
-            given = normalize_tuple_param(offsets, rank, "offsets")
-            if not all(isinstance(o, int) and -2 ** 62 < o < 2 ** 62 for o in given):
-                raise ValueError(f"offsets must be integers, got {offsets!r}")
-            origin = (ctypes.c_int64 * 3)(*given, *(0,) * (3 - rank))
-    spec = _spec(dims, base, frequencies, bool(interleaved))
-    if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad):
-        return _ag.rotary_with_grad(query, key, spec, origin, start, positions)
-    return _cuda.rotary(query, key, spec, origin, start, positions)
+    elif torch.is_tensor(offsets):
+        start = offsets
+    elif offsets is not None:
+        origin = normalize_tuple_param(offsets, rank, "offsets")
+        if not all(isinstance(o, int) and -2 ** 62 < o < 2 ** 62 for o in origin):
+            raise ValueError(f"offsets must be integers, got {offsets!r}")
+    spec = _spec(query.shape[-1], rank if positions is None else positions.shape[-1],
+                 None if axis_dims is None else tuple(axis_dims), float(base),
+                 None if frequencies is None else tuple(float(f) for f in frequencies), bool(interleaved))
+    return _lib.binding().rotary(query, key, spec, origin, start, positions)
 
 
 __all__ = ["rotary", "split_axis_dims"]
