@@ -3,12 +3,17 @@
 //   mean = sum x / C,  rstd = 1 / sqrt(sum (x - mean)^2 / C + eps),  xh = (x - mean) rstd,  y = xh w + b
 //   gw = dy w,  dx = rstd (gw - sum gw / C - xh sum(gw xh) / C),  dw = sum_rows dy xh,  db = sum_rows dy
 //
-// All of it is bound by memory: the forward reads x and writes y, the backward reads x and dy and writes dx.  A row
-// stays in the registers of the threads that own it (one load per element, the variance is taken about the mean and
-// not as a difference of squares), statistics and sums are float32, y and dx are rounded once.  The rows of dw and db
-// are summed by every thread for the columns it owns over all rows its block visits; the blocks' sums go to a scratch
-// buffer and a second kernel adds them in a fixed order, so that a result never depends on the order of atomics.
+// All of it is bound by memory: the forward reads x and writes y, the backward reads x and dy and writes dx.  A thread
+// owns the same few columns of all rows its block visits, so that the weights and the sums for dw and db stay in
+// registers; TPR threads share a row, and every thread has several rows in flight, which is what hides the latency of
+// memory between the two sums that a row needs before it can be written.  The variance is taken about the mean and not
+// as a difference of squares, statistics and sums are float32, y and dx are rounded once.  The blocks' sums for dw and db
+// go to a scratch buffer and a second kernel adds them in a fixed order, so that a result never depends on the order of
+// atomics.
 #include <math.h>
+
+#include <atomic>
+#include <type_traits>
 
 #include "launch.cuh"
 
@@ -83,188 +88,223 @@ __device__ __forceinline__ long long row_start(const NormArgs& a, uint32_t r) {
   return (long long)o * a.outer_stride + (long long)(r - o * a.inner) * a.inner_stride;
 }
 
-// Sum over the TPR threads of a row; every one of them gets it.  Rows wider than a warp are a whole block, `buf` has
-// a slot per warp, and two alternating buffers make one barrier per sum enough.
-template <int TPR>
-__device__ __forceinline__ float row_sum(float v, float* buf) {
+// Sums over the TPR threads of a row, for R rows at once; every thread gets them.  Rows wider than a warp meet in `buf`
+// [R][warps]: two buffers used in turn make one barrier per sum enough.
+template <int TPR, int R, int WARPS>
+__device__ __forceinline__ void row_sums(float (&v)[R], float (*buf)[WARPS]) {
   constexpr int W = TPR < 32 ? TPR : 32;
 #pragma unroll
-  for (int o = W / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int o = W / 2; o > 0; o >>= 1)
+#pragma unroll
+    for (int k = 0; k < R; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
   if constexpr (TPR > 32) {
-    const int warp = threadIdx.x >> 5;
-    if ((threadIdx.x & 31) == 0) buf[warp] = v;
+    constexpr int N = TPR / 32;
+    const int warp = threadIdx.x >> 5, first = warp / N * N;
+    if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+      for (int k = 0; k < R; ++k) buf[k][warp] = v[k];
+    }
     __syncthreads();
-    v = 0.f;
 #pragma unroll
-    for (int i = 0; i < TPR / 32; ++i) v += buf[i];
-  }
-  return v;
-}
-template <int TPR>
-__device__ __forceinline__ float2 row_sum2(float2 v, float2* buf) {
-  constexpr int W = TPR < 32 ? TPR : 32;
+    for (int k = 0; k < R; ++k) {
+      v[k] = 0.f;
 #pragma unroll
-  for (int o = W / 2; o > 0; o >>= 1) {
-    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+      for (int i = 0; i < N; ++i) v[k] += buf[k][first + i];
+    }
   }
-  if constexpr (TPR > 32) {
-    const int warp = threadIdx.x >> 5;
-    if ((threadIdx.x & 31) == 0) buf[warp] = v;
-    __syncthreads();
-    v = make_float2(0.f, 0.f);
-#pragma unroll
-    for (int i = 0; i < TPR / 32; ++i) { v.x += buf[i].x; v.y += buf[i].y; }
-  }
-  return v;
 }
 
-// TPR threads per row, NV accesses of VB bytes per thread.
+// The NV vectors of a row that a thread owns: columns (i * TPR + lane) * VE, zeros past the end and for rows that are not
+// there.
 template <typename T, int VB, int TPR, int NV>
-__global__ void __launch_bounds__(TPR > 128 ? TPR : 128)
-layer_norm_fwd(const NormArgs a) {
-  constexpr int VE = VB / (int)sizeof(T), RPB = TPR > 128 ? 1 : 128 / TPR;
+__device__ __forceinline__ void load_row(const T* row, int lane, int C, bool live, typename Raw<VB>::type (&raw)[NV]) {
   typedef typename Raw<VB>::type R;
-  __shared__ float buf[2][TPR / 32 + 1];
-  const int lane = threadIdx.x % TPR;
-  const uint32_t groups = (a.rows + RPB - 1) / RPB;
-  for (uint32_t gr = blockIdx.x; gr < groups; gr += gridDim.x) {
-    const uint32_t r = gr * RPB + threadIdx.x / TPR;
-    const bool live = r < a.rows;
-    const T* x = static_cast<const T*>(a.x) + (live ? row_start(a, r) : 0);
-    R raw[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int col = (i * TPR + lane) * VE;
-      if (live && col < a.C) raw[i] = __ldg(reinterpret_cast<const R*>(x + col));
-      else raw[i] = R{};
+  for (int i = 0; i < NV; ++i) {
+    const int col = (i * TPR + lane) * (VB / (int)sizeof(T));
+    raw[i] = live && col < C ? __ldg(reinterpret_cast<const R*>(row + col)) : R{};
+  }
+}
+
+// TPR threads per row, NV accesses of VB bytes per thread and row, R rows in flight.
+template <typename T, int VB, int TPR, int NV, int R>
+__global__ void __launch_bounds__(TPR > 64 ? TPR : 128)
+layer_norm_fwd(const NormArgs a) {
+  constexpr int VE = VB / (int)sizeof(T), E = NV * VE, BLOCK = TPR > 64 ? TPR : 128, GROUPS = BLOCK / TPR;
+  __shared__ float buf[2][R][BLOCK / 32];
+  const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
+  float w[E], b[E];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int col = (i * TPR + lane) * VE;
+#pragma unroll
+    for (int j = 0; j < VE; ++j) { w[i * VE + j] = 1.f; b[i * VE + j] = 0.f; }
+    if (col < a.C && a.weight != nullptr) load_weights<T, VE>(a.weight, a.w_f32, col, w + i * VE);
+    if (col < a.C && a.bias != nullptr) load_weights<T, VE>(a.bias, a.w_f32, col, b + i * VE);
+  }
+  typename Raw<VB>::type raw[R][NV], next[R][NV];
+  auto load = [&](uint32_t base) {
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      const uint32_t r = base + k * GROUPS + group;
+      load_row<T, VB, TPR, NV>(static_cast<const T*>(a.x) + (r < a.rows ? row_start(a, r) : 0), lane, a.C, r < a.rows, next[k]);
     }
-    float s = 0.f;
+  };
+  const uint32_t step = gridDim.x * (GROUPS * R);
+  load(blockIdx.x * (GROUPS * R));
+  for (uint32_t base = blockIdx.x * (GROUPS * R); base < a.rows; base += step) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      float f[VE];
-      unpack<T, VB>(raw[i], f);
+    for (int k = 0; k < R; ++k)
 #pragma unroll
-      for (int j = 0; j < VE; ++j) s += f[j];
-    }
-    const float mean = row_sum<TPR>(s, buf[0]) * a.inv_c;
-    float q = 0.f;
+      for (int i = 0; i < NV; ++i) raw[k][i] = next[k][i];
+    if (base + step < a.rows) load(base + step);             // on their way while these rows are worked on
+    float s[R];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      if ((i * TPR + lane) * VE < a.C) {
-        float f[VE];
-        unpack<T, VB>(raw[i], f);
-#pragma unroll
-        for (int j = 0; j < VE; ++j) q = fmaf(f[j] - mean, f[j] - mean, q);
-      }
-    }
-    const float rstd = 1.f / sqrtf(row_sum<TPR>(q, buf[1]) * a.inv_c + a.eps);
-    if (live) {
-      T* y = static_cast<T*>(a.y) + (long long)r * a.C;
+    for (int k = 0; k < R; ++k) {
+      s[k] = 0.f;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int col = (i * TPR + lane) * VE;
-        if (col < a.C) {
-          float f[VE], w[VE], b[VE];
-          unpack<T, VB>(raw[i], f);
-          if (a.weight != nullptr) load_weights<T, VE>(a.weight, a.w_f32, col, w);
-          if (a.bias != nullptr) load_weights<T, VE>(a.bias, a.w_f32, col, b);
+        float f[VE];
+        unpack<T, VB>(raw[k][i], f);
 #pragma unroll
-          for (int j = 0; j < VE; ++j) {
-            f[j] = (f[j] - mean) * rstd;
-            if (a.weight != nullptr) f[j] *= w[j];
-            if (a.bias != nullptr) f[j] += b[j];
-          }
-          *reinterpret_cast<R*>(y + col) = pack<T, VB>(f);
+        for (int j = 0; j < VE; ++j) s[k] += f[j];
+      }
+    }
+    row_sums<TPR, R, BLOCK / 32>(s, buf[0]);
+    float mean[R];
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      mean[k] = s[k] * a.inv_c;
+      s[k] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        float f[VE];
+        unpack<T, VB>(raw[k][i], f);
+        if ((i * TPR + lane) * VE < a.C) {
+#pragma unroll
+          for (int j = 0; j < VE; ++j) s[k] = fmaf(f[j] - mean[k], f[j] - mean[k], s[k]);
         }
       }
-      if (a.mean != nullptr && lane == 0) {
-        a.mean[r] = mean;
-        a.rstd[r] = rstd;
+    }
+    row_sums<TPR, R, BLOCK / 32>(s, buf[1]);
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      const uint32_t r = base + k * GROUPS + group;
+      const float rstd = 1.f / sqrtf(s[k] * a.inv_c + a.eps);
+      if (r < a.rows) {
+        T* y = static_cast<T*>(a.y) + (long long)r * a.C;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const int col = (i * TPR + lane) * VE;
+          if (col < a.C) {
+            float f[VE];
+            unpack<T, VB>(raw[k][i], f);
+#pragma unroll
+            for (int j = 0; j < VE; ++j) f[j] = fmaf((f[j] - mean[k]) * rstd, w[i * VE + j], b[i * VE + j]);
+            *reinterpret_cast<typename Raw<VB>::type*>(y + col) = pack<T, VB>(f);
+          }
+        }
+        if (a.mean != nullptr && lane == 0) {
+          a.mean[r] = mean[k];
+          a.rstd[r] = rstd;
+        }
       }
     }
   }
 }
 
-// dx of the rows and this block's sums of dw and db.  Rows wider than a warp are a whole block; otherwise a block of
-// 256 threads holds 256 / TPR rows at a time.
-template <typename T, int VB, int TPR, int NV>
-__global__ void __launch_bounds__(TPR > 256 ? TPR : (TPR > 32 ? TPR : 256))
+// Threads of a block of the backward: several rows side by side while that fits 256.
+constexpr int bwd_block(int tpr) { return tpr > 256 ? tpr : 256 / tpr * tpr; }
+
+// dx of the rows and this block's sums of dw and db.
+template <typename T, int VB, int TPR, int NV, int R>
+__global__ void __launch_bounds__(bwd_block(TPR))
 layer_norm_bwd(const NormArgs a) {
-  constexpr int VE = VB / (int)sizeof(T), BLOCK = TPR > 32 ? TPR : 256, RPB = BLOCK / TPR, E = NV * VE;
-  typedef typename Raw<VB>::type R;
-  __shared__ float2 buf[2][TPR / 32 + 1];
-  const int lane = threadIdx.x % TPR;
-  const uint32_t groups = (a.rows + RPB - 1) / RPB;
-  float dw[E], db[E];
+  constexpr int VE = VB / (int)sizeof(T), E = NV * VE, BLOCK = bwd_block(TPR), GROUPS = BLOCK / TPR, WARPS = BLOCK / 32;
+  __shared__ float buf[2][2 * R][WARPS];
+  const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // the joining kernel may be set up meanwhile
+  float w[E], dw[E], db[E];
 #pragma unroll
-  for (int j = 0; j < E; ++j) dw[j] = db[j] = 0.f;
-  int flip = 0;
-  for (uint32_t gr = blockIdx.x; gr < groups; gr += gridDim.x, flip ^= 1) {
-    const uint32_t r = gr * RPB + threadIdx.x / TPR;
-    const bool live = r < a.rows;
-    const T* x = static_cast<const T*>(a.x) + (live ? row_start(a, r) : 0);
-    const T* dy = static_cast<const T*>(a.dy) + (live ? (long long)r * a.C : 0);
-    R rx[NV], rg[NV];
+  for (int i = 0; i < NV; ++i) {
+    const int col = (i * TPR + lane) * VE;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int col = (i * TPR + lane) * VE;
-      if (live && col < a.C) {
-        rx[i] = __ldg(reinterpret_cast<const R*>(x + col));
-        rg[i] = __ldg(reinterpret_cast<const R*>(dy + col));
-      } else {
-        rx[i] = R{};
-        rg[i] = R{};
-      }
+    for (int j = 0; j < VE; ++j) { w[i * VE + j] = 1.f; dw[i * VE + j] = db[i * VE + j] = 0.f; }
+    if (col < a.C && a.weight != nullptr) load_weights<T, VE>(a.weight, a.w_f32, col, w + i * VE);
+  }
+  typename Raw<VB>::type rx[R][NV], rg[R][NV], nx[R][NV], ng[R][NV];
+  float mean[R], rstd[R], nmean[R], nrstd[R];
+  auto load = [&](uint32_t base) {
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      const uint32_t r = base + k * GROUPS + group;
+      const bool live = r < a.rows;
+      load_row<T, VB, TPR, NV>(static_cast<const T*>(a.x) + (live ? row_start(a, r) : 0), lane, a.C, live, nx[k]);
+      load_row<T, VB, TPR, NV>(static_cast<const T*>(a.dy) + (live ? (long long)r * a.C : 0), lane, a.C, live, ng[k]);
+      nmean[k] = live ? a.mean[r] : 0.f;
+      nrstd[k] = live ? a.rstd[r] : 0.f;
     }
-    const float mean = live ? a.mean[r] : 0.f, rstd = live ? a.rstd[r] : 0.f;
-    float2 s = make_float2(0.f, 0.f);
+  };
+  int flip = 0;
+  const uint32_t step = gridDim.x * (GROUPS * R);
+  load(blockIdx.x * (GROUPS * R));
+  for (uint32_t base = blockIdx.x * (GROUPS * R); base < a.rows; base += step, flip ^= 1) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int col = (i * TPR + lane) * VE;
-      if (live && col < a.C) {
-        float f[VE], g[VE], w[VE];
-        unpack<T, VB>(rx[i], f);
-        unpack<T, VB>(rg[i], g);
-        if (a.weight != nullptr) load_weights<T, VE>(a.weight, a.w_f32, col, w);
+    for (int k = 0; k < R; ++k) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) { rx[k][i] = nx[k][i]; rg[k][i] = ng[k][i]; }
+      mean[k] = nmean[k];
+      rstd[k] = nrstd[k];
+    }
+    if (base + step < a.rows) load(base + step);             // on their way while these rows are worked on
+    float s[2 * R];
+    // columns past the end hold zeros in x and dy; dy = 0 keeps them out of all four sums
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      s[2 * k] = s[2 * k + 1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        float f[VE], g[VE];
+        unpack<T, VB>(rx[k][i], f);
+        unpack<T, VB>(rg[k][i], g);
 #pragma unroll
         for (int j = 0; j < VE; ++j) {
-          const float xh = (f[j] - mean) * rstd;
+          const float xh = (f[j] - mean[k]) * rstd[k], gw = g[j] * w[i * VE + j];
           dw[i * VE + j] = fmaf(g[j], xh, dw[i * VE + j]);
           db[i * VE + j] += g[j];
-          const float gw = a.weight != nullptr ? g[j] * w[j] : g[j];
-          s.x += gw;
-          s.y = fmaf(gw, xh, s.y);
+          s[2 * k] += gw;
+          s[2 * k + 1] = fmaf(gw, xh, s[2 * k + 1]);
         }
       }
     }
     if (a.dx != nullptr) {
-      s = row_sum2<TPR>(s, buf[flip]);
-      s.x *= a.inv_c;
-      s.y *= a.inv_c;
-      T* dx = static_cast<T*>(a.dx) + (long long)r * a.C;
+      row_sums<TPR, 2 * R, WARPS>(s, buf[flip]);
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int col = (i * TPR + lane) * VE;
-        if (live && col < a.C) {
-          float f[VE], g[VE], w[VE];
-          unpack<T, VB>(rx[i], f);
-          unpack<T, VB>(rg[i], g);
-          if (a.weight != nullptr) load_weights<T, VE>(a.weight, a.w_f32, col, w);
+      for (int k = 0; k < R; ++k) {
+        const uint32_t r = base + k * GROUPS + group;
+        const float c1 = s[2 * k] * a.inv_c, c2 = s[2 * k + 1] * a.inv_c;
+        T* dx = static_cast<T*>(a.dx) + (long long)r * a.C;
 #pragma unroll
-          for (int j = 0; j < VE; ++j) {
-            const float xh = (f[j] - mean) * rstd;
-            const float gw = a.weight != nullptr ? g[j] * w[j] : g[j];
-            f[j] = rstd * (gw - s.x - xh * s.y);
+        for (int i = 0; i < NV; ++i) {
+          const int col = (i * TPR + lane) * VE;
+          if (r < a.rows && col < a.C) {
+            float f[VE], g[VE];
+            unpack<T, VB>(rx[k][i], f);
+            unpack<T, VB>(rg[k][i], g);
+#pragma unroll
+            for (int j = 0; j < VE; ++j) {
+              const float xh = (f[j] - mean[k]) * rstd[k];
+              f[j] = rstd[k] * (fmaf(g[j], w[i * VE + j], -c1) - xh * c2);
+            }
+            *reinterpret_cast<typename Raw<VB>::type*>(dx + col) = pack<T, VB>(f);
           }
-          *reinterpret_cast<R*>(dx + col) = pack<T, VB>(f);
         }
       }
     }
   }
   if (a.part == nullptr) return;
   float* part = a.part + (size_t)blockIdx.x * 2 * a.C;
-  if constexpr (TPR > 32) {
+  if constexpr (GROUPS == 1) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int col = (i * TPR + lane) * VE;
@@ -277,47 +317,54 @@ layer_norm_bwd(const NormArgs a) {
       }
     }
   } else {
-    // the rows side by side in a warp, then the block's warps, in a fixed order
-    constexpr int WARPS = BLOCK / 32;
-    __shared__ float acc[WARPS][TPR * E];
-    const int warp = threadIdx.x >> 5;
+    // the rows side by side in a warp, then the groups of warps, in a fixed order
+    constexpr int ROWS = TPR < 32 ? WARPS : GROUPS;
+    __shared__ float acc[ROWS][TPR * E];
+    const int at = TPR < 32 ? threadIdx.x >> 5 : group;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      float* v = half == 0 ? dw : db;
+    for (int which = 0; which < 2; ++which) {
+      float* v = which == 0 ? dw : db;
 #pragma unroll
       for (int j = 0; j < E; ++j) {
         float t = v[j];
 #pragma unroll
         for (int o = 16; o >= TPR; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-        if ((threadIdx.x & 31) < TPR) acc[warp][((j / VE) * TPR + lane) * VE + j % VE] = t;
+        if (TPR >= 32 || (threadIdx.x & 31) < TPR) acc[at][((j / VE) * TPR + lane) * VE + j % VE] = t;
       }
       __syncthreads();
       for (int c = threadIdx.x; c < a.C; c += BLOCK) {
         float t = 0.f;
 #pragma unroll
-        for (int i = 0; i < WARPS; ++i) t += acc[i][c];
-        part[half * a.C + c] = t;
+        for (int i = 0; i < ROWS; ++i) t += acc[i][c];
+        part[which * a.C + c] = t;
       }
       __syncthreads();
     }
   }
 }
 
+// Sum over a block of 512 threads.
+__device__ __forceinline__ float block_sum(float v, float (*buf)[16]) {
+  float one[1] = {v};
+  row_sums<512, 1, 16>(one, buf);
+  return one[0];
+}
+
 // Rows too wide for registers: a block walks the row once per pass; the second and third pass find it in the L2.
 template <typename T>
 __global__ void __launch_bounds__(512) layer_norm_fwd_wide(const NormArgs a) {
-  __shared__ float buf[2][512 / 32 + 1];
+  __shared__ float buf[2][1][16];
   for (uint32_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
     const T* x = static_cast<const T*>(a.x) + row_start(a, r);
     float s = 0.f;
     for (int c = threadIdx.x; c < a.C; c += 512) s += to_f<T>(x[c]);
-    const float mean = row_sum<512>(s, buf[0]) * a.inv_c;
+    const float mean = block_sum(s, buf[0]) * a.inv_c;
     float q = 0.f;
     for (int c = threadIdx.x; c < a.C; c += 512) {
       const float d = to_f<T>(x[c]) - mean;
       q = fmaf(d, d, q);
     }
-    const float rstd = 1.f / sqrtf(row_sum<512>(q, buf[1]) * a.inv_c + a.eps);
+    const float rstd = 1.f / sqrtf(block_sum(q, buf[1]) * a.inv_c + a.eps);
     T* y = static_cast<T*>(a.y) + (long long)r * a.C;
     for (int c = threadIdx.x; c < a.C; c += 512) {
       float f = (to_f<T>(x[c]) - mean) * rstd, t;
@@ -334,27 +381,26 @@ __global__ void __launch_bounds__(512) layer_norm_fwd_wide(const NormArgs a) {
 
 template <typename T>
 __global__ void __launch_bounds__(512) layer_norm_bwd_wide(const NormArgs a) {
-  __shared__ float2 buf[2][512 / 32 + 1];
+  __shared__ float buf[2][2][16];
   int flip = 0;
   for (uint32_t r = blockIdx.x; r < a.rows; r += gridDim.x, flip ^= 1) {
     const T* x = static_cast<const T*>(a.x) + row_start(a, r);
     const T* dy = static_cast<const T*>(a.dy) + (long long)r * a.C;
     const float mean = a.mean[r], rstd = a.rstd[r];
-    float2 s = make_float2(0.f, 0.f);
+    float s[2] = {0.f, 0.f};
     for (int c = threadIdx.x; c < a.C; c += 512) {
       float gw = to_f<T>(dy[c]), t;
       if (a.weight != nullptr) { load_weights<T, 1>(a.weight, a.w_f32, c, &t); gw *= t; }
-      s.x += gw;
-      s.y = fmaf(gw, (to_f<T>(x[c]) - mean) * rstd, s.y);
+      s[0] += gw;
+      s[1] = fmaf(gw, (to_f<T>(x[c]) - mean) * rstd, s[1]);
     }
-    s = row_sum2<512>(s, buf[flip]);
-    s.x *= a.inv_c;
-    s.y *= a.inv_c;
+    row_sums<512, 2, 16>(s, buf[flip]);
+    const float c1 = s[0] * a.inv_c, c2 = s[1] * a.inv_c;
     T* dx = static_cast<T*>(a.dx) + (long long)r * a.C;
     for (int c = threadIdx.x; c < a.C; c += 512) {
       float gw = to_f<T>(dy[c]), t;
       if (a.weight != nullptr) { load_weights<T, 1>(a.weight, a.w_f32, c, &t); gw *= t; }
-      dx[c] = from_f<T>(rstd * (gw - s.x - (to_f<T>(x[c]) - mean) * rstd * s.y));
+      dx[c] = from_f<T>(rstd * (gw - c1 - (to_f<T>(x[c]) - mean) * rstd * c2));
     }
   }
 }
@@ -380,6 +426,7 @@ __global__ void __launch_bounds__(256) layer_norm_sums_wide(const NormArgs a) {
 template <typename W>
 __global__ void __launch_bounds__(1024)
 layer_norm_join(const float* __restrict__ part, int n, int C, W* __restrict__ dweight, W* __restrict__ dbias) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");      // for the end of the kernel that writes the sums
   __shared__ float s[32][33];
   const int half = blockIdx.y, c = blockIdx.x * 32 + threadIdx.x;
   W* out = half == 0 ? dweight : dbias;
@@ -400,15 +447,9 @@ layer_norm_join(const float* __restrict__ part, int n, int C, W* __restrict__ dw
 }
 
 constexpr int kSMs = 148;
+constexpr int kMostSums = kSMs * 4;      // blocks of a backward, and so the partial sums it writes
 
-// Blocks of the backward, and so the partial sums it writes.
-int bwd_blocks(uint32_t rows, int rows_per_block, int per_sm) {
-  const uint32_t groups = (rows + rows_per_block - 1) / rows_per_block;
-  const uint32_t most = kSMs * per_sm;
-  return (int)(groups < most ? groups : most);
-}
-
-// Widest access that the row length, the row starts and the tensors' alignment allow.
+// Widest access that the row length, the row starts and the tensors' alignment allow; 0 when elements are not aligned.
 int access_bytes(const NormArgs& a, int size) {
   uintptr_t all = (uintptr_t)a.x | (uintptr_t)a.y | (uintptr_t)a.dy | (uintptr_t)a.dx | (uintptr_t)a.weight |
                   (uintptr_t)a.bias | (uintptr_t)((long long)a.C * size) | (uintptr_t)(a.outer_stride * size) |
@@ -416,47 +457,75 @@ int access_bytes(const NormArgs& a, int size) {
   return all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : all % size == 0 ? 2 : 0;
 }
 
-template <typename T, int VB, int TPR, int E>
+// Blocks of a kernel that an SM holds, asked once.
+template <typename Kernel>
+int resident(Kernel kernel, int block, std::atomic<int>& cached) {
+  int n = cached.load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, block, 0) != cudaSuccess || n < 1) {
+      (void)cudaGetLastError();
+      n = 1;
+    }
+    cached.store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+template <typename T, int VB, int TPR>
 void launch_fwd(const NormArgs& a, cudaStream_t s) {
-  constexpr int BLOCK = TPR > 128 ? TPR : 128, NV = E * (int)sizeof(T) / VB;
-  const uint32_t groups = (a.rows + BLOCK / TPR - 1) / (BLOCK / TPR);
-  const uint32_t most = kSMs * (2048 / BLOCK);
-  NB_LAUNCH("layer_norm_fwd", s, layer_norm_fwd<T, VB, TPR, NV><<<groups < most ? groups : most, BLOCK, 0, s>>>(a));
+  constexpr int BLOCK = TPR > 64 ? TPR : 128, NV = 8 * (int)sizeof(T) / VB, R = TPR >= 512 ? 1 : 2, ROWS = BLOCK / TPR * R;
+  static std::atomic<int> cached{0};
+  const uint32_t blocks = (a.rows + ROWS - 1) / ROWS, most = kSMs * resident(layer_norm_fwd<T, VB, TPR, NV, R>, BLOCK, cached);
+  NB_LAUNCH("layer_norm_fwd", s, layer_norm_fwd<T, VB, TPR, NV, R><<<blocks < most ? blocks : most, BLOCK, 0, s>>>(a));
+}
+
+template <typename T, int VB, int TPR>
+int launch_bwd(const NormArgs& a, cudaStream_t s) {
+  constexpr int BLOCK = bwd_block(TPR), NV = 8 * (int)sizeof(T) / VB, R = TPR >= 512 ? 1 : 2, ROWS = BLOCK / TPR * R;
+  static std::atomic<int> cached{0};
+  const int fit = resident(layer_norm_bwd<T, VB, TPR, NV, R>, BLOCK, cached);
+  // two visits for each block at least: the sums that a block leaves cost about as much as three of its rows
+  const uint32_t blocks = (a.rows + 2 * ROWS - 1) / (2 * ROWS), most = kSMs * (fit < 4 ? fit : 4);
+  const int n = (int)(blocks < most ? blocks : most);
+  NB_LAUNCH("layer_norm_bwd", s, layer_norm_bwd<T, VB, TPR, NV, R><<<n, BLOCK, 0, s>>>(a));
+  return n;
+}
+
+// A row takes the fewest threads whose eight columns each cover it.  There are variants for accesses of 16 bytes up to
+// 2560 columns in steps of a half and a third, coarser ones beyond and for narrower accesses.
+template <typename T, int VB, typename Launch>
+int by_width(const NormArgs& a, Launch&& launch) {
+#define NB_WIDTH(limit, threads) if (a.C <= limit) return launch(std::integral_constant<int, threads>())
+  if constexpr (VB == 16) {
+    NB_WIDTH(32, 4);
+    NB_WIDTH(64, 8);
+    NB_WIDTH(128, 16);
+    NB_WIDTH(256, 32);
+    NB_WIDTH(512, 64);
+    NB_WIDTH(768, 96);
+    NB_WIDTH(1024, 128);
+    NB_WIDTH(1536, 192);
+    NB_WIDTH(2560, 320);
+  }
+  NB_WIDTH(64, 8);
+  NB_WIDTH(256, 32);
+  NB_WIDTH(1024, 128);
+  NB_WIDTH(4096, 512);
+  NB_WIDTH(8192, 1024);
+#undef NB_WIDTH
+  return 0;
 }
 
 template <typename T, int VB>
-bool fwd_by_width(const NormArgs& a, cudaStream_t s) {
-  if (a.C <= 32) launch_fwd<T, VB, 4, 8>(a, s);
-  else if (a.C <= 64) launch_fwd<T, VB, 8, 8>(a, s);
-  else if (a.C <= 128) launch_fwd<T, VB, 16, 8>(a, s);
-  else if (a.C <= 256) launch_fwd<T, VB, 32, 8>(a, s);
-  else if (a.C <= 512) launch_fwd<T, VB, 32, 16>(a, s);
-  else if (a.C <= 1024) launch_fwd<T, VB, 32, 32>(a, s);
-  else if (a.C <= 4096) launch_fwd<T, VB, 128, 32>(a, s);
-  else if (a.C <= 16384) launch_fwd<T, VB, 512, 32>(a, s);
-  else return false;
-  return true;
+int fwd_by_width(const NormArgs& a, cudaStream_t s) {
+  return by_width<T, VB>(a, [&](auto tpr) {
+    launch_fwd<T, VB, decltype(tpr)::value>(a, s);
+    return 1;
+  });
 }
-
-template <typename T, int VB, int TPR, int E>
-int launch_bwd(const NormArgs& a, cudaStream_t s) {
-  constexpr int BLOCK = TPR > 32 ? TPR : 256, NV = E * (int)sizeof(T) / VB;
-  const int blocks = bwd_blocks(a.rows, BLOCK / TPR, 1024 / BLOCK);
-  NB_LAUNCH("layer_norm_bwd", s, layer_norm_bwd<T, VB, TPR, NV><<<blocks, BLOCK, 0, s>>>(a));
-  return blocks;
-}
-
 template <typename T, int VB>
 int bwd_by_width(const NormArgs& a, cudaStream_t s) {
-  if (a.C <= 32) return launch_bwd<T, VB, 4, 8>(a, s);
-  if (a.C <= 64) return launch_bwd<T, VB, 8, 8>(a, s);
-  if (a.C <= 128) return launch_bwd<T, VB, 16, 8>(a, s);
-  if (a.C <= 256) return launch_bwd<T, VB, 32, 8>(a, s);
-  if (a.C <= 512) return launch_bwd<T, VB, 32, 16>(a, s);
-  if (a.C <= 1024) return launch_bwd<T, VB, 128, 8>(a, s);
-  if (a.C <= 2048) return launch_bwd<T, VB, 128, 16>(a, s);
-  if (a.C <= 8192) return launch_bwd<T, VB, 512, 16>(a, s);
-  return 0;
+  return by_width<T, VB>(a, [&](auto tpr) { return launch_bwd<T, VB, decltype(tpr)::value>(a, s); });
 }
 
 // Partial rows of the widths that take the wide kernels.
@@ -464,7 +533,7 @@ constexpr int kWideSlices = 64;
 
 template <typename T>
 int fwd(const NormArgs& a, cudaStream_t s) {
-  bool done;
+  int done;
   const int vb = access_bytes(a, sizeof(T));
   if (vb == 0) return set_error(NATTEN_B200_EINVAL, "layer_norm_forward: tensor pointers must be aligned to their elements");
   if (vb == 16) done = fwd_by_width<T, 16>(a, s);
@@ -498,8 +567,18 @@ int bwd(const NormArgs& a, void* dweight, void* dbias, cudaStream_t s) {
   if (int rc = check_launch("layer norm backward")) return rc;
   if (a.part == nullptr) return NATTEN_B200_OK;
   const dim3 grid((a.C + 31) / 32, 2), block(32, 32);
-  if (a.w_f32) NB_LAUNCH("layer_norm_join", s, layer_norm_join<float><<<grid, block, 0, s>>>(a.part, n, a.C, (float*)dweight, (float*)dbias));
-  else NB_LAUNCH("layer_norm_join", s, layer_norm_join<T><<<grid, block, 0, s>>>(a.part, n, a.C, (T*)dweight, (T*)dbias));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.stream = s;
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  const float* part = a.part;
+  if (a.w_f32) NB_LAUNCH("layer_norm_join", s, (void)cudaLaunchKernelEx(&cfg, layer_norm_join<float>, part, n, a.C, (float*)dweight, (float*)dbias));
+  else NB_LAUNCH("layer_norm_join", s, (void)cudaLaunchKernelEx(&cfg, layer_norm_join<T>, part, n, a.C, (T*)dweight, (T*)dbias));
   return check_launch("layer norm sums");
 }
 
@@ -545,8 +624,7 @@ int natten_b200_layer_norm_forward(int32_t dtype, int32_t weight_dtype, const na
 
 size_t natten_b200_layer_norm_backward_scratch_bytes(int64_t rows, int32_t channels) {
   if (rows < 1 || channels < 1) return 0;
-  // no more blocks than rows, and no more than a launch of the narrowest blocks has
-  const int64_t most = kSMs * 8;
+  const int64_t most = kMostSums;        // and no more blocks than rows
   return (size_t)(rows < most ? rows : most) * 2 * (size_t)channels * sizeof(float);
 }
 

@@ -81,7 +81,7 @@ def _case(x, w, b, g, eps=1e-5):
 
 # widths on both sides of the variants' limits, odd ones, and lengths from a single row
 WIDTHS = [(5, 1), (3, 2), (37, 7), (33, 32), (70, 33), (9, 64), (19, 96), (130, 128), (3, 200), (50, 256), (2, 257),
-          (17, 512), (5, 513), (40, 1000), (9, 1024), (4, 1025), (7, 2048), (3, 2056), (2, 4096), (3, 4100), (2, 8192),
+          (17, 512), (5, 513), (31, 768), (7, 776), (40, 1000), (9, 1024), (4, 1025), (6, 1536), (7, 2048), (3, 2056), (5, 2560), (2, 2568), (2, 4096), (3, 4100), (2, 8192),
           (2, 8200), (1, 16384), (2, 16385), (3, 20000)]
 
 
