@@ -15,6 +15,7 @@
 #include <atomic>
 #include <type_traits>
 
+#include "f32x2.cuh"
 #include "launch.cuh"
 
 namespace nb {
@@ -60,6 +61,21 @@ __device__ __forceinline__ void load_weights(const void* w, bool f32, int col, f
     constexpr int VB = N * (int)sizeof(T);
     unpack<T, VB>(__ldg(reinterpret_cast<const typename Raw<VB>::type*>(static_cast<const T*>(w) + col)), out);
   }
+}
+
+// A thread's share of the weights, `none` where there are none.
+template <typename T, int VE, int TPR, int NV>
+__device__ __forceinline__ void weight_row(const void* w, bool f32, int lane, int C, float none, f32x2 (&out)[NV * VE / 2]) {
+  float f[NV * VE];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int col = (i * TPR + lane) * VE;
+#pragma unroll
+    for (int j = 0; j < VE; ++j) f[i * VE + j] = none;
+    if (col < C && w != nullptr) load_weights<T, VE>(w, f32, col, f + i * VE);
+  }
+#pragma unroll
+  for (int j = 0; j < NV * VE / 2; ++j) out[j] = pair(f[2 * j], f[2 * j + 1]);
 }
 
 struct NormArgs {
@@ -126,6 +142,37 @@ __device__ __forceinline__ void load_row(const T* row, int lane, int C, bool liv
   }
 }
 
+// Pair j of a thread's share of a row with zeros for columns past the end.
+template <int VE, int TPR>
+__device__ __forceinline__ f32x2 there(f32x2 v, int j, int lane, int C) {
+  float lo, hi;
+  unpair(v, lo, hi);
+  return pair((2 * j / VE * TPR + lane) * VE < C ? lo : 0.f, ((2 * j + 1) / VE * TPR + lane) * VE < C ? hi : 0.f);
+}
+
+// The same as E / 2 pairs of float32.
+template <typename T, int VB, int NV>
+__device__ __forceinline__ void unpack_row(const typename Raw<VB>::type (&raw)[NV], f32x2 (&out)[NV * VB / (int)sizeof(T) / 2]) {
+  constexpr int VE = VB / (int)sizeof(T);
+  float f[NV * VE];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) unpack<T, VB>(raw[i], f + i * VE);
+#pragma unroll
+  for (int j = 0; j < NV * VE / 2; ++j) out[j] = pair(f[2 * j], f[2 * j + 1]);
+}
+template <typename T, int VB, int TPR, int NV>
+__device__ __forceinline__ void store_row(T* row, int lane, int C, const f32x2 (&v)[NV * VB / (int)sizeof(T) / 2]) {
+  constexpr int VE = VB / (int)sizeof(T);
+  float f[NV * VE];
+#pragma unroll
+  for (int j = 0; j < NV * VE / 2; ++j) unpair(v[j], f[2 * j], f[2 * j + 1]);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int col = (i * TPR + lane) * VE;
+    if (col < C) *reinterpret_cast<typename Raw<VB>::type*>(row + col) = pack<T, VB>(f + i * VE);
+  }
+}
+
 // TPR threads per row, NV accesses of VB bytes per thread and row, R rows in flight.
 template <typename T, int VB, int TPR, int NV, int R>
 __global__ void __launch_bounds__(TPR > 64 ? TPR : 128)
@@ -133,15 +180,10 @@ layer_norm_fwd(const NormArgs a) {
   constexpr int VE = VB / (int)sizeof(T), E = NV * VE, BLOCK = TPR > 64 ? TPR : 128, GROUPS = BLOCK / TPR;
   __shared__ float buf[2][R][BLOCK / 32];
   const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
-  float w[E], b[E];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int col = (i * TPR + lane) * VE;
-#pragma unroll
-    for (int j = 0; j < VE; ++j) { w[i * VE + j] = 1.f; b[i * VE + j] = 0.f; }
-    if (col < a.C && a.weight != nullptr) load_weights<T, VE>(a.weight, a.w_f32, col, w + i * VE);
-    if (col < a.C && a.bias != nullptr) load_weights<T, VE>(a.bias, a.w_f32, col, b + i * VE);
-  }
+  const bool full = ((NV - 1) * TPR + lane) * VE < a.C;      // all of the thread's columns are there
+  f32x2 w[E / 2], b[E / 2];
+  weight_row<T, VE, TPR, NV>(a.weight, a.w_f32, lane, a.C, 1.f, w);
+  weight_row<T, VE, TPR, NV>(a.bias, a.w_f32, lane, a.C, 0.f, b);
   typename Raw<VB>::type raw[R][NV], next[R][NV];
   auto load = [&](uint32_t base) {
 #pragma unroll
@@ -159,32 +201,29 @@ layer_norm_fwd(const NormArgs a) {
       for (int i = 0; i < NV; ++i) raw[k][i] = next[k][i];
     if (base + step < a.rows) load(base + step);             // on their way while these rows are worked on
     float s[R];
+    f32x2 f[R][E / 2];
 #pragma unroll
     for (int k = 0; k < R; ++k) {
-      s[k] = 0.f;
+      unpack_row<T, VB, NV>(raw[k], f[k]);
+      f32x2 t = f[k][0];
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        float f[VE];
-        unpack<T, VB>(raw[k][i], f);
-#pragma unroll
-        for (int j = 0; j < VE; ++j) s[k] += f[j];
-      }
+      for (int j = 1; j < E / 2; ++j) t = add2(t, f[k][j]);
+      s[k] = sum2(t);
     }
     row_sums<TPR, R, BLOCK / 32>(s, buf[0]);
     float mean[R];
 #pragma unroll
     for (int k = 0; k < R; ++k) {
       mean[k] = s[k] * a.inv_c;
-      s[k] = 0.f;
+      const f32x2 minus = pair(-mean[k], -mean[k]);
+      f32x2 t = 0ull;
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        float f[VE];
-        unpack<T, VB>(raw[k][i], f);
-        if ((i * TPR + lane) * VE < a.C) {
-#pragma unroll
-          for (int j = 0; j < VE; ++j) s[k] = fmaf(f[j] - mean[k], f[j] - mean[k], s[k]);
-        }
+      for (int j = 0; j < E / 2; ++j) {
+        f[k][j] = add2(f[k][j], minus);
+        if (!full) f[k][j] = there<VE, TPR>(f[k][j], j, lane, a.C);    // columns past the end stay out of the variance
+        t = fma2(f[k][j], f[k][j], t);
       }
+      s[k] = sum2(t);
     }
     row_sums<TPR, R, BLOCK / 32>(s, buf[1]);
 #pragma unroll
@@ -192,18 +231,10 @@ layer_norm_fwd(const NormArgs a) {
       const uint32_t r = base + k * GROUPS + group;
       const float rstd = 1.f / sqrtf(s[k] * a.inv_c + a.eps);
       if (r < a.rows) {
-        T* y = static_cast<T*>(a.y) + (long long)r * a.C;
+        const f32x2 scale = pair(rstd, rstd);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          const int col = (i * TPR + lane) * VE;
-          if (col < a.C) {
-            float f[VE];
-            unpack<T, VB>(raw[k][i], f);
-#pragma unroll
-            for (int j = 0; j < VE; ++j) f[j] = fmaf((f[j] - mean[k]) * rstd, w[i * VE + j], b[i * VE + j]);
-            *reinterpret_cast<typename Raw<VB>::type*>(y + col) = pack<T, VB>(f);
-          }
-        }
+        for (int j = 0; j < E / 2; ++j) f[k][j] = fma2(mul2(f[k][j], scale), w[j], b[j]);
+        store_row<T, VB, TPR, NV>(static_cast<T*>(a.y) + (long long)r * a.C, lane, a.C, f[k]);
         if (a.mean != nullptr && lane == 0) {
           a.mean[r] = mean[k];
           a.rstd[r] = rstd;
@@ -224,14 +255,10 @@ layer_norm_bwd(const NormArgs a) {
   __shared__ float buf[2][2 * R][WARPS];
   const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // the joining kernel may be set up meanwhile
-  float w[E], dw[E], db[E];
+  f32x2 w[E / 2], dw[E / 2], db[E / 2];
+  weight_row<T, VE, TPR, NV>(a.weight, a.w_f32, lane, a.C, 1.f, w);
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int col = (i * TPR + lane) * VE;
-#pragma unroll
-    for (int j = 0; j < VE; ++j) { w[i * VE + j] = 1.f; dw[i * VE + j] = db[i * VE + j] = 0.f; }
-    if (col < a.C && a.weight != nullptr) load_weights<T, VE>(a.weight, a.w_f32, col, w + i * VE);
-  }
+  for (int j = 0; j < E / 2; ++j) dw[j] = db[j] = 0ull;
   typename Raw<VB>::type rx[R][NV], rg[R][NV], nx[R][NV], ng[R][NV];
   float mean[R], rstd[R], nmean[R], nrstd[R];
   auto load = [&](uint32_t base) {
@@ -261,43 +288,36 @@ layer_norm_bwd(const NormArgs a) {
     // columns past the end hold zeros in x and dy; dy = 0 keeps them out of all four sums
 #pragma unroll
     for (int k = 0; k < R; ++k) {
-      s[2 * k] = s[2 * k + 1] = 0.f;
+      f32x2 f[E / 2], g[E / 2], s0 = 0ull, s1 = 0ull;
+      unpack_row<T, VB, NV>(rx[k], f);
+      unpack_row<T, VB, NV>(rg[k], g);
+      const f32x2 minus = pair(-mean[k], -mean[k]), scale = pair(rstd[k], rstd[k]);
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        float f[VE], g[VE];
-        unpack<T, VB>(rx[k][i], f);
-        unpack<T, VB>(rg[k][i], g);
-#pragma unroll
-        for (int j = 0; j < VE; ++j) {
-          const float xh = (f[j] - mean[k]) * rstd[k], gw = g[j] * w[i * VE + j];
-          dw[i * VE + j] = fmaf(g[j], xh, dw[i * VE + j]);
-          db[i * VE + j] += g[j];
-          s[2 * k] += gw;
-          s[2 * k + 1] = fmaf(gw, xh, s[2 * k + 1]);
-        }
+      for (int j = 0; j < E / 2; ++j) {
+        const f32x2 xh = mul2(add2(f[j], minus), scale), gw = mul2(g[j], w[j]);
+        dw[j] = fma2(g[j], xh, dw[j]);
+        db[j] = add2(db[j], g[j]);
+        s0 = add2(s0, gw);
+        s1 = fma2(gw, xh, s1);
       }
+      s[2 * k] = sum2(s0);
+      s[2 * k + 1] = sum2(s1);
     }
     if (a.dx != nullptr) {
       row_sums<TPR, 2 * R, WARPS>(s, buf[flip]);
 #pragma unroll
       for (int k = 0; k < R; ++k) {
         const uint32_t r = base + k * GROUPS + group;
-        const float c1 = s[2 * k] * a.inv_c, c2 = s[2 * k + 1] * a.inv_c;
-        T* dx = static_cast<T*>(a.dx) + (long long)r * a.C;
+        if (r < a.rows) {
+          const float c1 = -s[2 * k] * a.inv_c, c2 = -s[2 * k + 1] * a.inv_c;
+          const f32x2 minus = pair(-mean[k], -mean[k]), scale = pair(rstd[k], rstd[k]), p1 = pair(c1, c1), p2 = pair(c2, c2);
+          f32x2 f[E / 2], g[E / 2];
+          unpack_row<T, VB, NV>(rx[k], f);
+          unpack_row<T, VB, NV>(rg[k], g);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          const int col = (i * TPR + lane) * VE;
-          if (r < a.rows && col < a.C) {
-            float f[VE], g[VE];
-            unpack<T, VB>(rx[k][i], f);
-            unpack<T, VB>(rg[k][i], g);
-#pragma unroll
-            for (int j = 0; j < VE; ++j) {
-              const float xh = (f[j] - mean[k]) * rstd[k];
-              f[j] = rstd[k] * (fmaf(g[j], w[i * VE + j], -c1) - xh * c2);
-            }
-            *reinterpret_cast<typename Raw<VB>::type*>(dx + col) = pack<T, VB>(f);
-          }
+          for (int j = 0; j < E / 2; ++j)
+            f[j] = mul2(scale, fma2(mul2(add2(f[j], minus), scale), p2, fma2(g[j], w[j], p1)));
+          store_row<T, VB, TPR, NV>(static_cast<T*>(a.dx) + (long long)r * a.C, lane, a.C, f);
         }
       }
     }
@@ -306,16 +326,15 @@ layer_norm_bwd(const NormArgs a) {
   float* part = a.part + (size_t)blockIdx.x * 2 * a.C;
   if constexpr (GROUPS == 1) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int col = (i * TPR + lane) * VE;
-      if (col < a.C) {
+    for (int which = 0; which < 2; ++which)
 #pragma unroll
-        for (int j = 0; j < VE; ++j) {
-          part[col + j] = dw[i * VE + j];
-          part[a.C + col + j] = db[i * VE + j];
-        }
+      for (int j = 0; j < E / 2; ++j) {
+        float lo, hi;
+        unpair(which == 0 ? dw[j] : db[j], lo, hi);
+        const int c0 = (2 * j / VE * TPR + lane) * VE + 2 * j % VE, c1 = ((2 * j + 1) / VE * TPR + lane) * VE + (2 * j + 1) % VE;
+        if (c0 < a.C) part[which * a.C + c0] = lo;
+        if (c1 < a.C) part[which * a.C + c1] = hi;
       }
-    }
   } else {
     // the rows side by side in a warp, then the groups of warps, in a fixed order
     constexpr int ROWS = TPR < 32 ? WARPS : GROUPS;
@@ -323,7 +342,9 @@ layer_norm_bwd(const NormArgs a) {
     const int at = TPR < 32 ? threadIdx.x >> 5 : group;
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
-      float* v = which == 0 ? dw : db;
+      float v[E];
+#pragma unroll
+      for (int j = 0; j < E / 2; ++j) unpair(which == 0 ? dw[j] : db[j], v[2 * j], v[2 * j + 1]);
 #pragma unroll
       for (int j = 0; j < E; ++j) {
         float t = v[j];

@@ -14,6 +14,7 @@
 
 #include <type_traits>
 
+#include "f32x2.cuh"
 #include "fna_sm100.cuh"
 #include "prefix.cuh"
 #include "sm100_ptx.cuh"
@@ -76,24 +77,6 @@ __device__ __forceinline__ float ex2(float x) {
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-// Pairs of floats: one instruction for both.
-typedef unsigned long long f32x2;
-__device__ __forceinline__ f32x2 pair(float lo, float hi) {
-  f32x2 d;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
-  return d;
-}
-__device__ __forceinline__ void unpair(f32x2 v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-  f32x2 d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
-  f32x2 d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
 template <bool BF16>
