@@ -494,7 +494,7 @@ int resident(Kernel kernel, int block, std::atomic<int>& cached) {
 
 template <typename T, int VB, int TPR>
 void launch_fwd(const NormArgs& a, cudaStream_t s) {
-  constexpr int BLOCK = TPR > 64 ? TPR : 128, NV = 8 * (int)sizeof(T) / VB, R = TPR >= 512 ? 1 : 2, ROWS = BLOCK / TPR * R;
+  constexpr int BLOCK = TPR > 64 ? TPR : 128, NV = 8 * (int)sizeof(T) / VB, R = TPR > 512 ? 1 : 2, ROWS = BLOCK / TPR * R;
   static std::atomic<int> cached{0};
   const uint32_t blocks = (a.rows + ROWS - 1) / ROWS, most = kSMs * resident(layer_norm_fwd<T, VB, TPR, NV, R>, BLOCK, cached);
   NB_LAUNCH("layer_norm_fwd", s, layer_norm_fwd<T, VB, TPR, NV, R><<<blocks < most ? blocks : most, BLOCK, 0, s>>>(a));
@@ -502,7 +502,7 @@ void launch_fwd(const NormArgs& a, cudaStream_t s) {
 
 template <typename T, int VB, int TPR>
 int launch_bwd(const NormArgs& a, cudaStream_t s) {
-  constexpr int BLOCK = bwd_block(TPR), NV = 8 * (int)sizeof(T) / VB, R = TPR >= 512 ? 1 : 2, ROWS = BLOCK / TPR * R;
+  constexpr int BLOCK = bwd_block(TPR), NV = 8 * (int)sizeof(T) / VB, R = TPR > 512 ? 1 : 2, ROWS = BLOCK / TPR * R;
   static std::atomic<int> cached{0};
   const int fit = resident(layer_norm_bwd<T, VB, TPR, NV, R>, BLOCK, cached);
   // two visits for each block at least: the sums that a block leaves cost about as much as three of its rows

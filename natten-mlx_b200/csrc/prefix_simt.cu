@@ -19,6 +19,13 @@ namespace {
 constexpr int kSMs = 148;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
+// 2^x within two units of the last place.
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // Four elements of a row from column c as float32; zeros past D and for rows that do not exist.
 template <typename T>
 __device__ __forceinline__ float4 load4(const T* row, int c, int D, bool vec, bool live) {
@@ -82,18 +89,32 @@ __global__ void __launch_bounds__(256) prefix_simt(const PrefixArgs a, bool vec)
     for (int j = 0; j < NJ; ++j) o[i][j] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
   const float sc = a.scale * kLog2e;
+  // The next tile's keys and values are on their way in registers while this one is worked on.
+  constexpr int Q4 = 16 * NJ, N4 = BN * Q4 / 256;          // float4 of a row, and of a tile for each thread
+  float4 nk[N4], nv[N4];
+  auto fetch = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < N4; ++i) {
+      const int at = threadIdx.x + i * 256, r = at / Q4, c = at % Q4 * 4;
+      const long long key = (long long)t * BN + r;
+      const bool live = key < a.prefix && c < a.D;
+      nk[i] = load4<T>(static_cast<const T*>(a.k) + (live ? key * a.k_token : 0) + (long long)hk * a.k_head, c, a.D, vec, live);
+      nv[i] = load4<T>(static_cast<const T*>(a.v) + (live ? key * a.v_token : 0) + (long long)hk * a.v_head, c, a.D, vec, live);
+    }
+  };
+  if (t0 < t1) fetch(t0);
   for (int t = t0; t < t1; ++t) {
     const int key0 = t * BN;
     if (!__syncthreads_or(most > key0)) break;       // also: the last tile's reads are over
-    for (int i = threadIdx.x; i < BN * (Dp / 4); i += 256) {
-      const int r = i / (Dp / 4), c = (i - r * (Dp / 4)) * 4;
-      const long long key = key0 + r;
-      const bool live = key < a.prefix;
-      *reinterpret_cast<float4*>(ks + r * LD + c) =
-          load4<T>(static_cast<const T*>(a.k) + (live ? key : 0) * a.k_token + (long long)hk * a.k_head, c, a.D, vec, live);
-      *reinterpret_cast<float4*>(vs + r * Dp + c) =
-          load4<T>(static_cast<const T*>(a.v) + (live ? key : 0) * a.v_token + (long long)hk * a.v_head, c, a.D, vec, live);
+#pragma unroll
+    for (int i = 0; i < N4; ++i) {
+      const int at = threadIdx.x + i * 256, r = at / Q4, c = at % Q4 * 4;
+      if (c < Dp) {
+        *reinterpret_cast<float4*>(ks + r * LD + c) = nk[i];
+        *reinterpret_cast<float4*>(vs + r * Dp + c) = nv[i];
+      }
     }
+    if (t + 1 < t1) fetch(t + 1);
     __syncthreads();
     float s[RM][CN];
 #pragma unroll
@@ -124,12 +145,12 @@ __global__ void __launch_bounds__(256) prefix_simt(const PrefixArgs a, bool vec)
 #pragma unroll
       for (int w = 8; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
       const float mn = fmaxf(m[i], mx), base = mn == -INFINITY ? 0.f : mn;
-      const float alpha = exp2f(m[i] - base);
+      const float alpha = ex2(m[i] - base);
       m[i] = mn;
       float sum = 0.f;
 #pragma unroll
       for (int j = 0; j < CN; ++j) {
-        const float p = exp2f(s[i][j] - base);
+        const float p = ex2(s[i][j] - base);
         sum += p;
         ps[(ty + 16 * i) * (BN + 4) + tx + 16 * j] = p;
       }
