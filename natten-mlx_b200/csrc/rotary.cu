@@ -8,7 +8,16 @@
 // computes the cosines and sines of their pairs once into shared memory, and all heads of q and k use them.  The
 // angle is exact for any 32-bit position: f is held as a fraction of a turn in 64-bit fixed point, so that the integer
 // product pos * f wraps around at whole turns by itself, and only the fraction that is left becomes a float.
+//
+// Small heads are bound by instructions before they are bound by memory: 100352 tokens of 8 heads of 32 (bf16) took 7000
+// thread instructions a token and 32 us while every 16 bytes worked out their own address and every pair its position
+// and an exact sincospif; 22 us now (15.7 us of memory at 6.5 TB/s).  589824 tokens of 32 heads of 64: 750 us, 98 % of
+// the copy rate.  Four units in flight per thread where a unit is one access, two where it is two (32 registers of data
+// either way): one in flight costs 15 % at these heads of 64.  Blocks for four per SM: eight leave the last round of
+// runs half empty at 100352 tokens (24.5 us).
 #include <math.h>
+
+#include <algorithm>
 
 #include "launch.cuh"
 
@@ -17,7 +26,8 @@ namespace {
 
 constexpr int kMaxPairs = 256;
 constexpr int kTable = 1024;     // (token, pair) entries of a block's table: 8 KB
-constexpr int kThreads = 256;
+constexpr int kRun = 256;        // most tokens of a run
+constexpr int kThreads = 256;    // most threads of a block
 constexpr int kSMs = 148;
 
 // Division of n < 2^31 by an invariant d >= 1 (Granlund and Montgomery, 1994): n * m >> (31 + s) with
@@ -43,8 +53,9 @@ struct RotaryArgs {
   int kind, pos64, pos_batch, inverse;
   int pairs, axis_end[3];                       // pairs of axis a end at axis_end[a]
   int tile;                                     // tokens of a block's run
-  FastDiv by_sample, by_ext[3], by_pairs, by_token, by_head;
-  uint32_t units_token, units_head;             // work units of a token and of a head
+  FastDiv by_sample, by_ext[3], by_pairs, by_lanes, by_head;
+  int units_token, units_head;                  // work units (16 bytes, two halves, or a pair) of a token and of a head
+  int passes, lanes, step;                      // threads for a token, passes over its units, tokens at a time
   uint64_t phase[kMaxPairs];
 };
 
@@ -73,86 +84,141 @@ __device__ __forceinline__ long long position(const RotaryArgs& a, uint32_t toke
   return p;
 }
 
-template <typename T, int MODE>
+// Cosine and sine of a number of half turns in [-1, 1).  For 16-bit types the fast instructions: their error, below
+// 2^-20, is far less than the rounding of the result (2^-12 and 2^-9 of it).
+template <typename T>
+__device__ __forceinline__ float2 cos_sin(float half_turns) {
+  float2 r;
+  if constexpr (sizeof(T) == 4) sincospif(half_turns, &r.y, &r.x);
+  else __sincosf(half_turns * 3.14159265358979f, &r.y, &r.x);
+  return r;
+}
+
+// A thread keeps its place in a token (head and channels) for a whole pass over the run and goes from token to token, so
+// that no address costs a division; it reads U tokens' channels before it works on the first, and the first ones before
+// the run's table is there.
+template <typename T, int MODE, int U>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryArgs a) {
   constexpr int VE = 16 / (int)sizeof(T);
-  constexpr bool HALVES = MODE == MODE_PAIRS_HALVES;
-  __shared__ uint64_t phase[kMaxPairs];
+  constexpr bool VEC = MODE == MODE_VEC_INTERLEAVED || MODE == MODE_VEC_HALVES, HALVES = MODE == MODE_VEC_HALVES || MODE == MODE_PAIRS_HALVES;
+  __shared__ long long pos[kRun * 3];
   __shared__ float2 table[kTable];
-  for (int i = threadIdx.x; i < a.pairs; i += kThreads) phase[i] = a.phase[i];
-  __syncthreads();
-  const int half = a.pairs;                    // rotated channels: 2 * pairs
+  const int pairs = a.pairs, tid = threadIdx.x, threads = blockDim.x;          // 2 * pairs channels are rotated
   const uint32_t runs = (a.tokens + a.tile - 1) / a.tile;
+  // the table: pairs next to each other, `step` tokens at a time
+  const int step = max(threads / pairs, 1), t_first = pairs <= threads ? (int)a.by_pairs.div(tid) : 0, p_first = tid - t_first * pairs;
+  auto axis_of = [&](int p) { return p < a.axis_end[0] ? 0 : p < a.axis_end[1] ? 1 : 2; };
+  auto entry = [&](long long at, uint64_t phase) {
+    // the top half of the fraction, read as signed: half turns in [-1, 1) after scaling
+    float2 c = cos_sin<T>((float)(int)(((uint64_t)at * phase) >> 32) * 4.656612873077393e-10f);
+    if (a.inverse) c.y = -c.y;
+    return c;
+  };
+  const uint64_t own_phase = p_first < pairs ? a.phase[p_first] : 0;
   for (uint32_t run = blockIdx.x; run < runs; run += gridDim.x) {
     const uint32_t first = run * a.tile;
-    const uint32_t n = min((uint32_t)a.tile, a.tokens - first);
-    for (uint32_t e = threadIdx.x; e < n * a.pairs; e += kThreads) {
-      const uint32_t t = a.by_pairs.div(e);
-      const int p = (int)(e - t * a.pairs);
-      const int axis = p < a.axis_end[0] ? 0 : p < a.axis_end[1] ? 1 : 2;
-      // the top half of the fraction, read as signed: half turns in [-1, 1) after scaling
-      const int frac = (int)(((uint64_t)position(a, first + t, axis) * phase[p]) >> 32);
-      float sn, cs;
-      sincospif((float)frac * 4.656612873077393e-10f, &sn, &cs);
-      table[e] = make_float2(cs, a.inverse ? -sn : sn);
-    }
-    __syncthreads();
-    for (uint32_t u = threadIdx.x; u < n * a.units_token; u += kThreads) {
-      const uint32_t t = a.by_token.div(u), in_token = u - t * a.units_token;
-      const uint32_t hh = a.by_head.div(in_token);
-      const int v = (int)(in_token - hh * a.units_head);
-      const bool is_q = hh < (uint32_t)a.heads_q;
+    const int n = (int)min((uint32_t)a.tile, a.tokens - first);
+    for (int pass = 0; pass < a.passes; ++pass) {
+      const int t_own = pass == 0 ? (int)a.by_lanes.div(tid) : 0, lane = tid - t_own * a.lanes, in_token = pass * a.lanes + lane;
+      const bool idle = t_own >= a.step || lane >= a.lanes || in_token >= a.units_token;
+      const int hh = (int)a.by_head.div(in_token), v = in_token - hh * a.units_head;
+      const bool is_q = hh < a.heads_q;
       const int h = is_q ? hh : hh - a.heads_q;
-      const uint32_t token = first + t;
-      const T* src = is_q ? static_cast<const T*>(a.q) + (long long)token * a.q_token + (long long)h * a.q_head
-                          : static_cast<const T*>(a.k) + (long long)token * a.k_token + (long long)h * a.k_head;
-      T* dst = is_q ? static_cast<T*>(a.yq) + ((long long)token * a.heads_q + h) * a.D
-                    : static_cast<T*>(a.yk) + ((long long)token * a.heads_k + h) * a.D;
-      const float2* cs = table + t * a.pairs;
-      if constexpr (MODE == MODE_VEC_INTERLEAVED) {
-        float f[VE];
-        load16<T>(src + v * VE, f);
+      const long long token = (long long)first + t_own, in = is_q ? a.q_token : a.k_token, out = (long long)(is_q ? a.heads_q : a.heads_k) * a.D;
+      const T* src = static_cast<const T*>(is_q ? a.q : a.k) + token * in + h * (is_q ? a.q_head : a.k_head);
+      T* dst = static_cast<T*>(is_q ? a.yq : a.yk) + token * out + (long long)h * a.D;
+      // channels of the unit: [c0, c0 + VE) and, for two halves, [c1, c1 + VE); without vectors two channels
+      const int rot = MODE == MODE_VEC_HALVES ? pairs / VE : MODE == MODE_VEC_INTERLEAVED ? a.units_head : pairs;
+      const bool turns = v < rot;
+      const int c0 = VEC ? (MODE == MODE_VEC_HALVES && !turns ? 2 * pairs + (v - rot) * VE : v * VE) : !turns ? v + pairs : HALVES ? v : 2 * v;
+      const int c1 = HALVES ? c0 + pairs : c0 + 1;
+      src += c0;
+      dst += c0;
+      const int end = idle ? 0 : n;
+      const long long in_step = in * a.step, out_step = out * a.step;
+      int t = t_own;
+      do {                                                 // at least once: the table is made inside
+        uint4 raw[U][2];
+        T one[U][2];
 #pragma unroll
-        for (int j = 0; j < VE / 2; ++j) {
-          const int p = v * (VE / 2) + j;
-          if (p < a.pairs) {
-            const float2 c = cs[p];
-            const float x = f[2 * j], y = f[2 * j + 1];
-            f[2 * j] = x * c.x - y * c.y;
-            f[2 * j + 1] = x * c.y + y * c.x;
+        for (int i = 0; i < U; ++i)
+          if (t + i * a.step < end) {
+            const T* x = src + i * in_step;
+            if constexpr (VEC) {
+              raw[i][0] = *reinterpret_cast<const uint4*>(x);
+              if (HALVES && turns) raw[i][1] = *reinterpret_cast<const uint4*>(x + pairs);
+            } else {
+              one[i][0] = x[0];
+              if (turns) one[i][1] = x[c1 - c0];
+            }
           }
+        if (pass == 0 && t == t_own) {
+          if (n * pairs <= threads) {                      // an entry for each thread: it finds its position by itself
+            if (t_first < n) table[tid] = entry(position(a, first + t_first, axis_of(p_first)), own_phase);
+          } else {
+            for (int i = tid; i < n * a.axes; i += threads) {
+              const int tt = i / a.axes;
+              pos[i] = position(a, first + tt, i - tt * a.axes);
+            }
+            __syncthreads();
+            for (int p = p_first; p < pairs; p += threads) {
+              const int axis = axis_of(p);
+              const uint64_t phase = p == p_first ? own_phase : a.phase[p];
+              if (t_first < step)
+                for (int tt = t_first; tt < n; tt += step) table[tt * pairs + p] = entry(pos[tt * a.axes + axis], phase);
+            }
+          }
+          __syncthreads();
         }
-        store16<T>(dst + v * VE, f);
-      } else if constexpr (MODE == MODE_VEC_HALVES) {
-        const int rot = half / VE;
-        float f[VE], g[VE];
-        if (v < rot) {
-          load16<T>(src + v * VE, f);
-          load16<T>(src + half + v * VE, g);
 #pragma unroll
-          for (int j = 0; j < VE; ++j) {
-            const float2 c = cs[v * VE + j];
-            const float x = f[j], y = g[j];
-            f[j] = x * c.x - y * c.y;
-            g[j] = x * c.y + y * c.x;
+        for (int i = 0; i < U; ++i)
+          if (t + i * a.step < end) {
+            const float2* cs = table + (t + i * a.step) * pairs;
+            T* y = dst + i * out_step;
+            if constexpr (MODE == MODE_VEC_INTERLEAVED) {
+              float f[VE];
+              load16<T>(reinterpret_cast<const T*>(&raw[i][0]), f);
+#pragma unroll
+              for (int j = 0; j < VE / 2; ++j) {
+                const int p = v * (VE / 2) + j;
+                if (p < pairs) {
+                  const float2 c = cs[p];
+                  const float x0 = f[2 * j], x1 = f[2 * j + 1];
+                  f[2 * j] = x0 * c.x - x1 * c.y;
+                  f[2 * j + 1] = x0 * c.y + x1 * c.x;
+                }
+              }
+              store16<T>(y, f);
+            } else if constexpr (MODE == MODE_VEC_HALVES) {
+              if (turns) {
+                float f[VE], g[VE];
+                load16<T>(reinterpret_cast<const T*>(&raw[i][0]), f);
+                load16<T>(reinterpret_cast<const T*>(&raw[i][1]), g);
+#pragma unroll
+                for (int j = 0; j < VE; ++j) {
+                  const float2 c = cs[v * VE + j];
+                  const float x0 = f[j], x1 = g[j];
+                  f[j] = x0 * c.x - x1 * c.y;
+                  g[j] = x0 * c.y + x1 * c.x;
+                }
+                store16<T>(y, f);
+                store16<T>(y + pairs, g);
+              } else {
+                *reinterpret_cast<uint4*>(y) = raw[i][0];
+              }
+            } else if (turns) {
+              const float2 c = cs[v];
+              const float x0 = to_f<T>(one[i][0]), x1 = to_f<T>(one[i][1]);
+              y[0] = from_f<T>(x0 * c.x - x1 * c.y);
+              y[c1 - c0] = from_f<T>(x0 * c.y + x1 * c.x);
+            } else {
+              y[0] = one[i][0];
+            }
           }
-          store16<T>(dst + v * VE, f);
-          store16<T>(dst + half + v * VE, g);
-        } else {
-          const int c = 2 * half + (v - rot) * VE;
-          *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(src + c);
-        }
-      } else {
-        if (v < half) {
-          const int i0 = HALVES ? v : 2 * v, i1 = HALVES ? v + half : 2 * v + 1;
-          const float2 c = cs[v];
-          const float x = to_f<T>(src[i0]), y = to_f<T>(src[i1]);
-          dst[i0] = from_f<T>(x * c.x - y * c.y);
-          dst[i1] = from_f<T>(x * c.y + y * c.x);
-        } else {
-          dst[v + half] = src[v + half];
-        }
-      }
+        src += U * in_step;
+        dst += U * out_step;
+        t += U * a.step;
+      } while (t < end);
     }
     __syncthreads();
   }
@@ -162,19 +228,24 @@ template <typename T>
 int launch(RotaryArgs& a, int mode, int units_head, cudaStream_t s) {
   a.units_head = units_head;
   a.units_token = units_head * (a.heads_q + a.heads_k);
-  a.by_head = FastDiv(a.units_head);
-  a.by_token = FastDiv(a.units_token);
+  // the lanes of a token, in as many passes as it needs, and as many tokens at a time as the block has room for
+  a.passes = (a.units_token + kThreads - 1) / kThreads;
+  a.lanes = (a.units_token + a.passes - 1) / a.passes;
+  a.step = a.passes > 1 ? 1 : kThreads / a.lanes;
+  const int threads = (a.lanes * a.step + 31) / 32 * 32;
   a.by_pairs = FastDiv(a.pairs);
-  // as many tokens as the table holds, but no fewer than four runs for each SM while there are so many tokens
-  const uint32_t spread = (a.tokens + kSMs * 4 - 1) / (kSMs * 4);
-  a.tile = (int)(spread < (uint32_t)(kTable / a.pairs) ? spread : (uint32_t)(kTable / a.pairs));
-  const uint32_t runs = (a.tokens + a.tile - 1) / a.tile, most = kSMs * 8;
+  a.by_lanes = FastDiv(a.lanes);
+  a.by_head = FastDiv(a.units_head);
+  // as many tokens as the table holds, but runs for all blocks while there are so many tokens, and as many for each
+  const uint32_t room = std::min(kTable / a.pairs, kRun), most = kSMs * 4, rounds = (uint32_t)((a.tokens + (uint64_t)most * room - 1) / ((uint64_t)most * room));
+  a.tile = (int)((a.tokens + (uint64_t)most * rounds - 1) / ((uint64_t)most * rounds));
+  const uint32_t runs = (a.tokens + a.tile - 1) / a.tile;
   const int grid = (int)(runs < most ? runs : most);
   switch (mode) {
-    case MODE_VEC_INTERLEAVED: NB_LAUNCH("rotary", s, rotary_kernel<T, MODE_VEC_INTERLEAVED><<<grid, kThreads, 0, s>>>(a)); break;
-    case MODE_VEC_HALVES: NB_LAUNCH("rotary", s, rotary_kernel<T, MODE_VEC_HALVES><<<grid, kThreads, 0, s>>>(a)); break;
-    case MODE_PAIRS_HALVES: NB_LAUNCH("rotary", s, rotary_kernel<T, MODE_PAIRS_HALVES><<<grid, kThreads, 0, s>>>(a)); break;
-    default: NB_LAUNCH("rotary", s, rotary_kernel<T, MODE_PAIRS><<<grid, kThreads, 0, s>>>(a)); break;
+    case MODE_VEC_INTERLEAVED: NB_LAUNCH("rotary", s, rotary_kernel<T, MODE_VEC_INTERLEAVED, 4><<<grid, threads, 0, s>>>(a)); break;
+    case MODE_VEC_HALVES: NB_LAUNCH("rotary", s, rotary_kernel<T, MODE_VEC_HALVES, 2><<<grid, threads, 0, s>>>(a)); break;
+    case MODE_PAIRS_HALVES: NB_LAUNCH("rotary", s, rotary_kernel<T, MODE_PAIRS_HALVES, 4><<<grid, threads, 0, s>>>(a)); break;
+    default: NB_LAUNCH("rotary", s, rotary_kernel<T, MODE_PAIRS, 4><<<grid, threads, 0, s>>>(a)); break;
   }
   return check_launch("rotary");
 }
