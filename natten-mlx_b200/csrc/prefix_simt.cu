@@ -249,11 +249,11 @@ __global__ void __launch_bounds__(W * 32, (W == 8 && NH <= 2 ? 2 : 1)) prefix_si
 // Joins the parts of a row and the window's result: 4 columns per lane, and where a row leaves lanes over they take other
 // parts; WARPS warps share a row's parts.  The order of the sums is fixed.  The kernel starts while the one that writes
 // the parts still runs, and waits for its end.
-constexpr int kMostParts = 256;
+constexpr int kMostParts = 256, kFewParts = 8;     // fewer than kFewParts: a warp per row
 
 template <typename T, int WARPS>
 __global__ void __launch_bounds__(128) prefix_join(const PrefixArgs a, int lanes) {
-  __shared__ float weight[4 / WARPS][WARPS == 1 ? 8 : kMostParts];
+  __shared__ float weight[4 / WARPS][WARPS == 1 ? kFewParts : kMostParts];
   __shared__ float4 sums[WARPS][64];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, of = warp % WARPS, slot = warp / WARPS;
@@ -382,7 +382,7 @@ int join(const PrefixArgs& a, cudaStream_t s) {
   cfg.numAttrs = 1;
   // four warps share a row's parts when each gets two or more (37 parts of 512 rows x 128: 4.0 us against 12 us for a
   // warp per row; two parts of 13312 rows x 128: 16 us for a warp per row against 30 us)
-  if (a.splits >= 8) {
+  if (a.splits >= kFewParts) {
     cfg.gridDim = dim3((unsigned)a.part_rows);
     NB_LAUNCH("prefix_join", s, (void)cudaLaunchKernelEx(&cfg, prefix_join<T, 4>, a, lanes));
   } else {
