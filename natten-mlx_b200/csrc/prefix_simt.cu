@@ -380,8 +380,8 @@ int join(const PrefixArgs& a, cudaStream_t s) {
   early.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &early;
   cfg.numAttrs = 1;
-  // four warps share a row's parts when each gets two or more (37 parts of 512 rows x 128: 4.0 us against 12 us for a
-  // warp per row; two parts of 13312 rows x 128: 16 us for a warp per row against 30 us)
+  // Four warps share a row's parts when each gets two or more: 37 parts of 512 rows x 128 11 us between events instead of
+  // 21 us.  With fewer parts a warp has a row: two parts of 16384 rows x 64 16 us instead of 40 us.  (Events add 8 us.)
   if (a.splits >= kFewParts) {
     cfg.gridDim = dim3((unsigned)a.part_rows);
     NB_LAUNCH("prefix_join", s, (void)cudaLaunchKernelEx(&cfg, prefix_join<T, 4>, a, lanes));

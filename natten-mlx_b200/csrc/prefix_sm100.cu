@@ -1,14 +1,29 @@
 // Attention to a shared prefix on the tensor cores (bf16, fp16).
 //
 // The queries of one key/value head, over all samples, positions and heads of its group, are the rows of one product,
-// so the prefix is read once for the batch.  A block owns two tiles of up to 128 rows and a range of 128-key chunks:
+// so the prefix is read once for the batch.  A block owns two tiles of up to 128 rows and a range of the prefix in chunks
+// of 96 keys (head dims to 64) or 128:
 //   TMA warp       Q tiles once, then K and V chunks into a ring of shared-memory slots (zero fill past the ends)
 //   MMA warp       S = Q K^T into tensor memory, O += P V with P from tensor memory (over S) and V MN-major
-//   16 softmax warps   eight per tile, two threads per row, each with half of the chunk's keys: the row's maximum, P =
-//                  2^(scale S - m) rounded to the tensors' type, the sum in float32; O stays in tensor memory throughout
+//   softmax warps  a thread per row, or two (head dims to 64) that share the chunk's keys: the row's maximum, P =
+//                  2^(scale S - m) rounded to the tensors' type, which the tensor core needs, the sum in float32; O stays
+//                  in tensor memory throughout
 // While one tile's softmax runs the tensor core works for the other tile.  A block that has one tile only lets its two
 // halves take every other chunk for it.  The reference maximum m of a row follows the true one lazily: O and the sum are
 // rescaled only when a chunk exceeds m by 2^8, so that P stays finite in either type.
+//
+// What bounds it, and what was measured (bf16, 4096 keys):
+// - Heads of 128, 16384 rows of 8 heads: 255 us, 1078 TFLOP/s, 66 % of the rate of a large library matrix product.  The
+//   tensor core is the bound, kept waiting at the ends of a block and by the one thread that issues its products.
+// - Heads of 64, 16384 rows of 16 heads: 391 us, 703 TFLOP/s, 43 %.  The products alone would take 234 us (P V of
+//   64 columns fills half of what the unit does at 128), the exponentials alone 239 us (16 per SM and clock), and the two
+//   overlap in part only: a chunk is 96 keys so that two buffers of S for each tile fit tensor memory, and Q K^T of the
+//   next chunk runs under this one's softmax.  Slower were: one buffer and 192 keys, two blocks per SM with chunks of 64
+//   keys, S read twice instead of kept, a second warp that issues products, and a part of the exponentials as polynomials.
+// - Two threads per row: heads of 64 391 us, one 409 us; heads of 128 268 us, one 255 us (with 128 keys of S in its
+//   registers a thread has no room for a second buffer's, and the pair's exchange of maxima costs more than it gives).
+// - Few rows: 128 rows of 4 heads of 128 over 65536 keys (fp16) 40 us, of which the 134 MB of keys and values need 21 us;
+//   the first S is there after 5 us, the parts' results and their joining take 7 us.
 #include <cuda.h>
 #include <math.h>
 
@@ -27,7 +42,7 @@ using namespace sm100;
 constexpr int kSMs = 148;
 constexpr int kRows = 128;               // rows of a tile = lanes of tensor memory
 constexpr int kSteps = 8;               // barriers of the ring, by step
-// For heads padded to DP channels: keys of a chunk, threads per row and keys of each, buffers of S / P for a tile, and the
+// For heads padded to DP channels: keys of a chunk, buffers of S / P for a tile, threads per row and keys of each, and the
 // threads of a block (the softmax warps of two tiles, a warp that loads, a warp that issues the products).
 template <int DP> struct Shape {
   static constexpr int kKeys = DP == 64 ? 96 : 128, kBufs = DP == 64 ? 2 : 1, kSplit = DP == 64 ? 2 : 1, kEach = kKeys / kSplit;
