@@ -83,6 +83,13 @@ void* stream_of(const at::Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.
 
 bool wants_grad(const at::Tensor& t) { return t.defined() && t.requires_grad(); }
 
+// There are no formulas for forward-mode differentiation: a tangent is refused, not dropped.
+template <typename... Tensors>
+void check_no_tangent(const char* name, const Tensors&... ts) {
+  const bool any = ((ts.defined() && ts._fw_grad(/*level=*/0).defined()) || ...);
+  TORCH_CHECK(!any, name, " does not support forward-mode differentiation");
+}
+
 void* ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 // Results of a backward pass that is recorded itself (create_graph): usable, but not to be differentiated again.
@@ -202,12 +209,13 @@ void check_vector(const char* name, const at::Tensor& t, const at::Tensor& x) {
 }
 
 at::Tensor layer_norm(const at::Tensor& x, const OptTensor& weight_opt, const OptTensor& bias_opt, double eps) {
+  const at::Tensor weight = weight_opt.value_or(at::Tensor()), bias = bias_opt.value_or(at::Tensor());
+  check_no_tangent("layer_norm", x, weight, bias);
   check_cuda(x);
   TORCH_CHECK_VALUE(dtype_code(x) >= 0, "unsupported dtype ", x.scalar_type(), "; expected float32, float16 or bfloat16");
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1, "layer_norm expects [..., C] with C >= 1, got ", x.sizes());
   TORCH_CHECK_VALUE(x.size(-1) <= INT32_MAX, "layer_norm expects fewer than 2^31 channels");
   TORCH_CHECK_VALUE(eps >= 0.0 && std::isfinite(eps), "eps must be finite and not negative, got ", eps);
-  const at::Tensor weight = weight_opt.value_or(at::Tensor()), bias = bias_opt.value_or(at::Tensor());
   if (weight.defined()) check_vector("weight", weight, x);
   if (bias.defined()) check_vector("bias", bias, x);
   TORCH_CHECK_VALUE(!weight.defined() || !bias.defined() || weight.scalar_type() == bias.scalar_type(),
@@ -354,6 +362,10 @@ std::pair<at::Tensor, at::Tensor> rotary(const at::Tensor& q, const at::Tensor& 
   TORCH_CHECK_VALUE(q.size(-1) == k.size(-1), "Head dim must match: Q has ", q.size(-1), ", K has ", k.size(-1), ".");
   TORCH_CHECK_VALUE(dtype_code(q) >= 0 && q.scalar_type() == k.scalar_type(),
                     "query and key must share a dtype of float32, float16 or bfloat16, got ", q.scalar_type(), " and ", k.scalar_type());
+  TORCH_CHECK_VALUE(q.size(-2) >= 1 && k.size(-2) >= 1, "query and key must have heads, got ", q.size(-2), " and ", k.size(-2));
+  for (int64_t i = 1; i < nd; ++i)
+    TORCH_CHECK_VALUE(q.size(i) <= INT32_MAX && k.size(i) <= INT32_MAX, "rotary expects sizes below 2^31, got ", q.sizes(), " and ", k.sizes());
+  check_no_tangent("rotary", q, k);
   check_cuda(q);
   TORCH_CHECK_VALUE(k.device() == q.device(), "query and key must be on one device");
   const int64_t axes = (int64_t)spec->axis_dims.size();
@@ -436,6 +448,7 @@ std::pair<at::Tensor, at::Tensor> prefix(const at::Tensor& q, const at::Tensor& 
     grad = grad || wants_grad(*window_out) || wants_grad(*window_lse);
   }
   TORCH_CHECK_VALUE(!scale.has_value() || (*scale > 0.0 && std::isfinite(*scale)), "scale must be positive and finite, got ", scale.value_or(0.0), ".");
+  check_no_tangent("prefix_attention", q, k, v, window_out.value_or(at::Tensor()), window_lse.value_or(at::Tensor()));
   TORCH_CHECK(!(at::GradMode::is_enabled() && grad),
               "prefix_attention computes no gradients: call it under torch.no_grad(), or detach its inputs");
   check_cuda(q);

@@ -82,6 +82,8 @@ def rotary(query: torch.Tensor, key: torch.Tensor, axis_dims: Optional[Sequence[
     if positions is not None:
         if offsets is not None:
             raise ValueError("offsets and positions cannot be combined")
+        if not torch.is_tensor(positions) or positions.dim() < 1:
+            raise ValueError("positions must be an int32 or int64 tensor with a last axis of coordinates")
     elif torch.is_tensor(offsets):
         start = offsets
     elif offsets is not None:

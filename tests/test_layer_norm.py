@@ -102,6 +102,20 @@ def test_many_rows(rows, c, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("c", [65, 66, 127, 130, 333, 334, 511, 514, 1026, 2001, 2046, 2050])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_narrow_accesses(c, dtype):
+    """Row lengths that leave accesses of 2 and 4 bytes, and so do rows that start off the wider boundaries."""
+    x = _rand((301, c), 1, dtype, 1.5, 0.4)
+    w, b, g = _rand((c,), 2, torch.float32, 0.3, 1.0), _rand((c,), 3, torch.float32, 0.3), _rand((301, c), 4, dtype)
+    y, grads = _case(x, w, b, g)
+    xs = torch.zeros(301, c + 3, dtype=dtype, device=DEV)[:, 1:c + 1].copy_(x).requires_grad_(True)
+    _check("y", nb.layer_norm(xs, w.to(DEV), b.to(DEV)), _definition(x, w, b, g, 1e-5)["y"])
+    ds, = torch.autograd.grad(nb.layer_norm(xs, w.to(DEV), b.to(DEV)), xs, g.to(DEV))
+    _check("dx", ds, _definition(x, w, b, g, 1e-5)["dx"])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("with_w,with_b", [(False, False), (True, False), (False, True)])
 def test_without_weights(with_w, with_b):
     c = 72
@@ -235,6 +249,14 @@ def test_double_backward_is_refused():
 
 
 # ---- refusals: nothing is launched -------------------------------------------------------------------------------
+
+def test_tangents_are_refused():
+    x, w = torch.zeros(2, 4), torch.ones(4)
+    with torch.autograd.forward_ad.dual_level():
+        for args in ((torch.autograd.forward_ad.make_dual(x, x), w), (x, torch.autograd.forward_ad.make_dual(w, w))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                nb.layer_norm(*args)
+
 
 def test_python_refusals():
     with pytest.raises(RuntimeError, match="CUDA tensors only"):

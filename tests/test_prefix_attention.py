@@ -144,6 +144,16 @@ def test_samples_that_see_a_part(dtype, path, window):
     _case((3, 50, 6, 40), 3, 300, dtype, path, lens=[0, 300, -4], window=window)
     _case((2, 150, 2, 128), 1, 260, dtype, path, lens=[130, 3], window=window)
     _case((3, 2, 2, 32), 1, 4000, dtype, path, lens=[0, 0, 0], window=window)
+    _case((9, 1, 3, 24), 3, 700, dtype, path, lens=[700, 3, 64, 65, 0, 62, 699, 1, 130], window=window)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [17, 28, 60, 124, 200])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_cuda_core_kernel_with_samples_that_see_a_part(d, dtype):
+    """Rows of one thread that end at different places, in head dims of every variant and at every bank of a row."""
+    _case((7, 3, 6, d), 2, 300, dtype, "simt", lens=[300, 1, 64, 31, 0, 33, 298])
+    _case((2, 5, 2, d), 2, 90, dtype, "simt", lens=[7, 90], window=True)
 
 
 @pytest.mark.gpu
@@ -279,6 +289,13 @@ def test_lens_in_64_bits_and_no_queries():
 
 
 # ---- refusals ----------------------------------------------------------------------------------------------------
+
+def test_tangents_are_refused():
+    q, k = torch.zeros(2, 5, 4, 8), torch.zeros(7, 2, 8)
+    with torch.autograd.forward_ad.dual_level(), torch.no_grad():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            nb.prefix_attention(q, torch.autograd.forward_ad.make_dual(k, k), k)
+
 
 def test_python_refusals():
     q, k = torch.zeros(2, 5, 4, 8), torch.zeros(7, 2, 8)

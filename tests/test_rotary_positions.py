@@ -3,7 +3,9 @@ strided inputs, refusals.
 
 Tolerance.  A result is a cos - b sin.  The angle, a fraction of a turn, is truncated to 2^-32 of a turn and rounded to 24
 bits of at most half a turn: 1.9e-7 radians; cosine and sine are within two units of the last place, 1.2e-7 below 1;
-the products and their sum add 2^-23 (|a| + |b|).  Together less than 2^-21 (|a| + |b|), and the result is rounded once."""
+the products and their sum add 2^-23 (|a| + |b|).  Together less than 2^-21 (|a| + |b|), and the result is rounded once.
+For 16-bit types the angle is rounded once more, as radians (1.9e-7), and cosine and sine are off by at most 2^-21.19 and
+2^-21.41: 1.9e-7 + 1.9e-7 + 4.2e-7 + 1.2e-7 = 9.2e-7, less than 2^-20 (9.5e-7)."""
 
 from __future__ import annotations
 
@@ -20,6 +22,7 @@ from natten_mlx_b200.positions import _phases, split_axis_dims
 
 DEV = "cuda"
 U = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+TURN = {torch.float32: 2.0 ** -21, torch.float16: 2.0 ** -20, torch.bfloat16: 2.0 ** -20}
 
 
 def _rand(shape, seed, dtype):
@@ -66,7 +69,7 @@ def _check(got, t, turns, interleaved, sign=1.0, angle_err=0.0):
     want, size, width = _turned(t, turns, interleaved, sign)
     got64 = got.detach().double().cpu()
     assert got.dtype == t.dtype and got.shape == t.shape and got.is_contiguous()
-    bound = U[got.dtype] * want.abs() + size * (2.0 ** -21 + angle_err) + (2.0 ** -25 if got.dtype == torch.float16 else 0.0)
+    bound = U[got.dtype] * want.abs() + size * (TURN[got.dtype] + angle_err) + (2.0 ** -25 if got.dtype == torch.float16 else 0.0)
     off = (got64 - want).abs()
     assert bool((off <= bound).all()), f"{float((off / bound).max()):.3g} of the bound"
     assert torch.equal(got[..., width:].cpu(), t.detach()[..., width:].cpu())
@@ -109,6 +112,23 @@ CASES = [
 def test_grid_positions(lead, hq, hk, d, dims, interleaved, dtype):
     q, k = _rand(lead + (hq, d), 1, dtype), _rand(lead + (hk, d), 2, dtype)
     _case(q, k, _turns(_grid(lead), dims), lambda a, b: nb.rotary(a, b, dims, interleaved=interleaved), interleaved)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lead,hq,hk,d,dims", [
+    ((1, 5, 4), 5, 4, 512, (256, 256)),      # a token's channels take several passes of the block, fewer threads than pairs
+    ((1, 700), 40, 9, 128, (128,)), ((2, 40, 41), 3, 2, 72, (36, 36)), ((1, 20011), 1, 1, 2, (2,)),
+])
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_wide_tokens_and_long_runs(lead, hq, hk, d, dims, interleaved, dtype):
+    q, k = _rand(lead + (hq, d), 1, dtype), _rand(lead + (hk, d), 2, dtype)
+    _case(q, k, _turns(_grid(lead), dims), lambda a, b: nb.rotary(a, b, dims, interleaved=interleaved), interleaved)
+    # heads that start off the 16-byte boundaries take the pairs one by one
+    q1, k1 = (_rand(lead + (h, d + 1), 3, dtype).to(DEV)[..., 1:] for h in (hq, hk))
+    yq, yk = nb.rotary(q1, k1, dims, interleaved=interleaved)
+    _check(yq, q1, _turns(_grid(lead), dims), interleaved)
+    _check(yk, k1, _turns(_grid(lead), dims), interleaved)
 
 
 @pytest.mark.gpu
@@ -235,6 +255,20 @@ def test_python_refusals():
                         ((q, k.half()), "dtype"), ((q.double(), k.double()), "dtype")]:
         with pytest.raises(ValueError, match=match):
             nb.rotary(*args)
+    with pytest.raises(ValueError, match="must have heads"):
+        nb.rotary(q[:, :, :0], k)
+    with pytest.raises(ValueError, match="must have heads"):
+        nb.rotary(q, k[:, :, :0])
+    many = torch.zeros(1, 1, 1, 2).expand(1, 2 ** 32 + 5, 1, 2)
+    with pytest.raises(ValueError, match="below 2"):
+        nb.rotary(many, many)
+    with pytest.raises(ValueError, match="positions must be"):
+        nb.rotary(q, k, positions=[0, 1, 2, 3, 4])
+    with pytest.raises(ValueError, match="positions must be"):
+        nb.rotary(q, k, positions=torch.tensor(3))
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            nb.rotary(torch.autograd.forward_ad.make_dual(q, torch.ones_like(q)), k)
     with pytest.raises(ValueError, match="rotary needs"):
         nb.nn.NeighborhoodAttention2D(12, 4, 3, rotary=True)
 
