@@ -187,3 +187,38 @@ def test_modules_can_be_copied_and_loaded():
     x = torch.randn(1, 5, 6, 16, device="cuda")
     with torch.no_grad():
         assert torch.equal(m(norm(x)), n(norm(x)))
+
+
+@pytest.mark.gpu
+def test_rows_further_apart_than_32_bits_reach():
+    """Views whose last rows start past 2^31 elements give the bits of their dense copies."""
+    far = 2 ** 30
+    room = torch.empty(2 * far + 8192, dtype=torch.bfloat16, device="cuda")
+
+    def apart(dense):
+        view = room.as_strided(dense.shape, (far,) + dense.stride()[1:])
+        return view.copy_(dense)
+
+    gen = torch.Generator("cuda").manual_seed(5)
+    x = torch.randn(3, 1000, generator=gen, device="cuda").bfloat16()
+    w = torch.randn(1000, generator=gen, device="cuda")
+    g = torch.randn(3, 1000, generator=gen, device="cuda").bfloat16()
+    got, want = [], []
+    for rows, results in ((apart(x), got), (x, want)):
+        rows = rows.detach().requires_grad_(True)
+        y = nb.layer_norm(rows, w)
+        results += [y.detach(), *torch.autograd.grad(y, rows, g)]
+    qk = torch.randn(3, 2, 64, generator=gen, device="cuda").bfloat16()
+    got += [nb.rotary(apart(qk)[None], qk[None])[0], nb.rotary(qk[None], apart(qk)[None])[1]]
+    want += [nb.rotary(qk[None], qk[None])[0]] * 2
+    q = torch.randn(2, 5, 4, 64, generator=gen, device="cuda").bfloat16()
+    for path in ("tcgen05", "simt"):
+        nb.set_fused_path(path)
+        try:
+            got += [nb.prefix_attention(q, apart(qk), qk), nb.prefix_attention(q, qk, apart(qk)),
+                    nb.prefix_attention(apart(qk)[None], qk, qk)]
+            want += [nb.prefix_attention(q, qk, qk)] * 2 + [nb.prefix_attention(qk[None], qk, qk)]
+        finally:
+            nb.set_fused_path("auto")
+    for i, (a, b) in enumerate(zip(got, want)):
+        assert torch.equal(a, b), i
