@@ -615,6 +615,9 @@ int bwd(const NormArgs& a, void* dweight, void* dbias, cudaStream_t s) {
   return check_launch("layer norm sums");
 }
 
+// Whether a pointer (null included) may be read as elements of `size` bytes.
+bool aligned_to(const void* p, int size) { return (uintptr_t)p % size == 0; }
+
 int check_rows(const char* what, int32_t dtype, int32_t wdtype, const natten_b200_rows* rows, NormArgs* a) {
   if (rows == nullptr) return set_error(NATTEN_B200_EINVAL, "%s: rows is null", what);
   if (dtype < NATTEN_B200_F32 || dtype > NATTEN_B200_BF16) return set_error(NATTEN_B200_EINVAL, "%s: unsupported dtype %d", what, dtype);
@@ -622,6 +625,7 @@ int check_rows(const char* what, int32_t dtype, int32_t wdtype, const natten_b20
     return set_error(NATTEN_B200_EINVAL, "%s: weights must have the tensor's dtype or be float32", what);
   if (rows->channels < 1) return set_error(NATTEN_B200_EINVAL, "%s: channels must be positive", what);
   if (rows->rows < 0 || rows->rows > 0x7fffffffLL) return set_error(NATTEN_B200_EINVAL, "%s: rows must be in [0, 2^31)", what);
+  if (rows->reserved != 0) return set_error(NATTEN_B200_EINVAL, "%s: reserved must be zero", what);
   if (rows->inner < 1 || rows->inner > 0x7fffffffLL) return set_error(NATTEN_B200_EINVAL, "%s: inner must be in [1, 2^31)", what);
   a->rows = (uint32_t)rows->rows;
   a->C = rows->channels;
@@ -649,6 +653,9 @@ int natten_b200_layer_norm_forward(int32_t dtype, int32_t weight_dtype, const na
   if (a.rows == 0) return NATTEN_B200_OK;
   if (x == nullptr || y == nullptr || (mean == nullptr) != (rstd == nullptr))
     return set_error(NATTEN_B200_EINVAL, "layer_norm_forward: null tensor");
+  const int ws = a.w_f32 ? 4 : 2;
+  if (!aligned_to(weight, ws) || !aligned_to(bias, ws) || !aligned_to(mean, 4) || !aligned_to(rstd, 4))
+    return set_error(NATTEN_B200_EINVAL, "layer_norm_forward: weights and statistics must be aligned to their elements");
   a.x = x; a.weight = weight; a.bias = bias; a.eps = eps; a.y = y; a.mean = mean; a.rstd = rstd;
   cudaStream_t s = (cudaStream_t)stream;
   if (dtype == NATTEN_B200_F32) return fwd<float>(a, s);
@@ -682,6 +689,9 @@ int natten_b200_layer_norm_backward(int32_t dtype, int32_t weight_dtype, const n
   if (sums && (scratch == nullptr || scratch_bytes < need || ((uintptr_t)scratch & 3) != 0))
     return set_error(NATTEN_B200_ERESOURCE, "layer_norm_backward: scratch has %zu bytes, needs %zu (4-byte aligned)",
                      scratch == nullptr ? (size_t)0 : scratch_bytes, need);
+  const int ws = a.w_f32 ? 4 : 2;
+  if (!aligned_to(weight, ws) || !aligned_to(dweight, ws) || !aligned_to(dbias, ws) || !aligned_to(mean, 4) || !aligned_to(rstd, 4))
+    return set_error(NATTEN_B200_EINVAL, "layer_norm_backward: weights and statistics must be aligned to their elements");
   a.x = x; a.weight = weight; a.mean = const_cast<float*>(mean); a.rstd = const_cast<float*>(rstd);
   a.dy = dy; a.dx = dx; a.part = sums ? static_cast<float*>(scratch) : nullptr;
   if (dtype == NATTEN_B200_F32) return bwd<float>(a, dweight, dbias, s);

@@ -484,6 +484,8 @@ int natten_b200_prefix_forward(const natten_b200_prefix_geom* g, const void* q, 
   if (((uintptr_t)scratch & 31) != 0) return set_error(NATTEN_B200_EINVAL, "prefix: scratch must be 32-byte aligned");
   for (const void* p : {q, k, v, (const void*)window_out, (const void*)out})
     if (((uintptr_t)p & 15) != 0) return set_error(NATTEN_B200_EINVAL, "prefix: tensor pointers must be 16-byte aligned");
+  if ((((uintptr_t)window_lse | (uintptr_t)lse | (uintptr_t)g->lens) & 3) != 0)
+    return set_error(NATTEN_B200_EINVAL, "prefix: lens, lse and window_lse must be aligned to their elements");
   bool tc;
   if (int rc = choose(g, &a, &tc)) return rc;
   const size_t need = scratch_bytes_of(a);

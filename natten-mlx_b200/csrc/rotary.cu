@@ -295,6 +295,8 @@ extern "C" int natten_b200_rotary(const natten_b200_rotary_geom* g, const void* 
   const int size = g->dtype == NATTEN_B200_F32 ? 4 : 2;
   const uintptr_t ptrs = (uintptr_t)q | (uintptr_t)k | (uintptr_t)yq | (uintptr_t)yk;
   if (ptrs % size != 0) return set_error(NATTEN_B200_EINVAL, "rotary: tensor pointers must be aligned to their elements");
+  if (g->position_kind != POS_GRID && (uintptr_t)g->positions % (g->position_bits / 8) != 0)
+    return set_error(NATTEN_B200_EINVAL, "rotary: positions must be aligned to their elements");
   a.q = q; a.k = k; a.yq = yq; a.yk = yk;
   a.q_token = g->q_token_stride; a.q_head = g->q_head_stride; a.k_token = g->k_token_stride; a.k_head = g->k_head_stride;
   a.positions = g->positions;

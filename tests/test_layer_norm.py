@@ -305,6 +305,22 @@ def test_abi_refusals(change, code, needle):
     assert _lib.launch_count() == before
 
 
+def test_abi_alignment_of_weights_and_statistics():
+    lib, before = _lib.load(), _lib.launch_count()
+    rows = _lib.Rows(4, 1, 8, 0, 8, 0)
+    for at, off in ((3, 2), (4, 2), (7, 2), (8, 1)):         # weight, bias (float32 beside bf16), mean, rstd
+        a = [_lib.BF16, _lib.F32, rows, 4096, 4096, 4096, 1e-5, 4096, 4096, 4096, None]
+        a[at + 1] += off
+        assert lib.natten_b200_layer_norm_forward(*a) == _lib.EINVAL and "aligned" in _lib.last_error()
+    for at, off in ((4, 2), (5, 2), (6, 2), (9, 2), (10, 2)):        # weight, mean, rstd, dweight, dbias
+        a = [_lib.BF16, _lib.F32, rows, 4096, 4096, 4096, 4096, 4096, 4096, 4096, 4096, 4096, 1 << 30, None]
+        a[at] += off
+        assert lib.natten_b200_layer_norm_backward(*a) == _lib.EINVAL and "aligned" in _lib.last_error()
+    assert lib.natten_b200_layer_norm_forward(_lib.BF16, _lib.F32, _lib.Rows(4, 1, 8, 0, 8, 1), 4096, 4096, 4096, 1e-5, 4096, 4096,
+                                              4096, None) == _lib.EINVAL and "reserved" in _lib.last_error()
+    assert _lib.launch_count() == before
+
+
 def test_abi_scratch_and_empty_calls():
     lib = _lib.load()
     rows = _lib.Rows(1000, 1, 64, 0, 64, 0)

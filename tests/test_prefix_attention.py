@@ -359,6 +359,9 @@ def test_abi_pointers_and_scratch():
     assert lib.natten_b200_prefix_forward(_geom(), None, 4096, 4096, None, None, 4096, None, None, 0, None) == _lib.EINVAL
     assert lib.natten_b200_prefix_forward(_geom(), 4096, 4096, 4096, 4096, None, 4096, None, None, 0, None) == _lib.EINVAL
     assert lib.natten_b200_prefix_forward(_geom(), 4096 + 8, 4096, 4096, None, None, 4096, None, None, 0, None) == _lib.EINVAL
+    for geom, wl, lse in ((_geom(lens=4096 + 2), 4096, 4096), (_geom(), 4096 + 1, 4096), (_geom(), 4096, 4096 + 2)):
+        assert lib.natten_b200_prefix_forward(geom, 4096, 4096, 4096, 4096, wl, 4096, lse, 4096, 1 << 40, None) == _lib.EINVAL
+        assert "aligned" in _lib.last_error()
     long = _geom(prefix=100000)
     need = lib.natten_b200_prefix_scratch_bytes(long)
     assert need > 0 and need % (65 * 4) == 0

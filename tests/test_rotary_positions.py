@@ -321,3 +321,6 @@ def test_abi_pointers():
     assert lib.natten_b200_rotary(_geom(), None, 4096, 4096, 4096, 0, None) == _lib.EINVAL
     assert lib.natten_b200_rotary(_geom(), 4096 + 2, 4096, 4096, 4096, 0, None) == _lib.EINVAL
     assert lib.natten_b200_rotary(_geom(batch=0), None, None, None, None, 0, None) == _lib.OK
+    assert lib.natten_b200_rotary(_geom(position_kind=1, positions=4096 + 2), 4096, 4096, 4096, 4096, 0, None) == _lib.EINVAL
+    assert lib.natten_b200_rotary(_geom(position_kind=2, position_bits=64, positions=4096 + 4), 4096, 4096, 4096, 4096, 0,
+                                  None) == _lib.EINVAL and "aligned" in _lib.last_error()
