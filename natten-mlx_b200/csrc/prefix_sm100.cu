@@ -21,8 +21,9 @@
 //   next chunk runs under this one's softmax.  Slower were: one buffer and 192 keys, two blocks per SM with chunks of 64
 //   keys, three tiles of one buffer each (406 us; the tiles wait for the same two units in turn, whichever their number),
 //   S read twice instead of kept, a second warp that issues products, a part of the exponentials as polynomials, and the
-//   two tiles taking turns at the exponentials by a barrier (436 us).  Without the exponentials it would take 294 us, and
-//   without the exchange of maxima between a row's two threads 366 us.
+//   two tiles taking turns at the exponentials by a barrier (436 us), and exponentials beside the maximum, with the
+//   reference so far, that are repeated where it does not hold (464 us: P can be handed over only after the check).
+//   Without the exponentials it would take 294 us, without the exchange of maxima between a row's two threads 366 us.
 // - Two threads per row: heads of 64 391 us, one 409 us; heads of 128 268 us, one 255 us (with 128 keys of S in its
 //   registers a thread has no room for a second buffer's, and the pair's exchange of maxima costs more than it gives).
 // - Few rows: 128 rows of 4 heads of 128 over 65536 keys (fp16) 40 us, of which the 134 MB of keys and values need 21 us;
